@@ -317,6 +317,53 @@ NCB_API int ncb_sample_rows_gather_device(NcbSampler* sampler, const float* d_lo
 NCB_API int ncb_softmax_rows_device(const float* d_in, float* d_out, int rows, int cols,
                                     void* stream);
 
+/* ---- sampling with options per row, min-p and 16-bit logits -----------------
+ * No reference counterpart (GenerationOptions has no min-p and the reference
+ * samples one row at a time, TokenSampler.cs:10). A serving batch: every row
+ * with its own options, logits as the LM head left them.
+ *
+ * Row of values x_i, i < vocab, with options T, k, p, m and a uniform u:
+ *   d_i = (x_i - max x) / T,  w_i = exp(d_i);  order: x descending, id ascending;
+ *   1. the first k values of the order (every finite value where k <= 0 or
+ *      k >= vocab), of mass Z;
+ *   2. of those the shortest prefix of mass >= p Z (all of them where p >= 1);
+ *   3. of those the values with w_i >= m (all of them where m = 0);
+ *   token = the first of the order whose prefix mass exceeds u times the mass
+ *   that is left. T = 0 takes the first maximum (greedy; u, k, p, m unread).
+ * Unlike ncb_sample_rows_device, which repeats the C# fp32 arithmetic and keeps
+ * every value equal to the k-th, this entry point keeps exactly k values and
+ * decides in (at least) 64-bit sums.
+ *
+ *   d_logits    [rows, vocab] of `dtype` (NCB_DTYPE_*), consecutive rows `ld`
+ *               elements apart (ld >= vocab); natural alignment suffices.
+ *               -inf: banned, never kept.
+ *   d_uniforms  rows fp32 in [0, 1)
+ *   d_temperature, d_top_k, d_top_p, d_min_p
+ *               rows values each, or NULL for 1, off, 1, 0 in every row.
+ *               T >= 0 and finite, 0 < p, 0 <= m <= 1.
+ *   d_tokens    rows int32 out
+ *   d_logprobs  rows fp32 out, or NULL: log of the probability the token was
+ *               drawn with, d_token - log(mass left); 0 for greedy rows
+ *   d_kept      rows int32 out, or NULL: how many values the draw chose from
+ *   d_flags     rows uint32 out, or NULL
+ * A row with a NaN or +inf value, or without a finite one, comes back as token
+ * -1 with NCB_FLAG_NONFINITE; one whose options or uniform are out of range as
+ * -1 with NCB_FLAG_BAD_OPTIONS (logprob NaN and kept 0 in both). Every other
+ * row is unaffected. Needs no handle and no scratch, keeps nothing between
+ * calls, and results do not depend on what else runs: calls may overlap on any
+ * streams and be captured. Runs on the current device; asynchronous on
+ * `stream`. rows = 0 is a no-op. vocab > 2^24: NCB_ERROR_CAPACITY. */
+#define NCB_DTYPE_F32 0
+#define NCB_DTYPE_F16 1
+#define NCB_DTYPE_BF16 2
+#define NCB_FLAG_BAD_OPTIONS 0x100u
+NCB_API int ncb_sample_rows_min_p_device(const void* d_logits, int dtype, int rows, int vocab,
+                                         int64_t ld, const float* d_uniforms,
+                                         const float* d_temperature, const int32_t* d_top_k,
+                                         const float* d_top_p, const float* d_min_p,
+                                         int32_t* d_tokens, float* d_logprobs, int32_t* d_kept,
+                                         uint32_t* d_flags, void* stream);
+
 /* ---- diagnostics ----------------------------------------------------------
  * Rows this handle has redone on the exact full-sort kernel since it was
  * created: top-k rows whose ties overflowed the candidate buffers, and

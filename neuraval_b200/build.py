@@ -26,6 +26,8 @@ UNITS = {
     "navsampler.cu": ["-fmad=false"],
     # the reference's softmax is compiled with nvcc's default contraction; so is ours
     "softmax_rows.cu": [],
+    # 64-bit sums decide; contraction only makes them more exact
+    "sample_min_p.cu": [],
 }
 def nvcc() -> str:
     cand = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "bin", "nvcc")

@@ -30,10 +30,15 @@ FLAG_EXP_SLOW = 0x10
 FLAG_BAD_HISTORY = 0x20
 FLAG_TIES_OVERFLOW = 0x40
 FLAG_PEER_TIMEOUT = 0x80
+FLAG_BAD_OPTIONS = 0x100
 # rows whose token may legitimately differ from the reference's
 PARITY_EXEMPT = FLAG_DRAW_BOUNDARY | FLAG_CUTOFF_BOUNDARY | FLAG_TIE_AT_DRAW
 
 INT_MAX = 2**31 - 1
+
+DTYPE_F32 = 0
+DTYPE_F16 = 1
+DTYPE_BF16 = 2
 
 
 class NcbSamplerParams(ctypes.Structure):
@@ -52,6 +57,7 @@ class NcbSamplerParams(ctypes.Structure):
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
+_L = ctypes.c_int64
 SIGNATURES = {
     "ncb_sampler_params_validate": (_I, [ctypes.POINTER(NcbSamplerParams)]),
     "ncb_sampler_create": (_I, [_I, _I, _I, _I, ctypes.POINTER(_P)]),
@@ -84,6 +90,8 @@ SIGNATURES = {
     "ncb_sample_rows_gather_device": (_I, [_P, _P, _I, _I, _I, _P, _P, _P,
                                            ctypes.POINTER(NcbSamplerParams), _P, _P, _P]),
     "ncb_softmax_rows_device": (_I, [_P, _P, _I, _I, _P]),
+    "ncb_sample_rows_min_p_device": (_I, [_P, _I, _I, _I, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P,
+                                          _P]),
     "ncb_logits_repetition_penalty": (_I, [_P, _P, _I, _I, _P, _P, _F]),
     "ncb_logits_frequency_presence_penalty": (_I, [_P, _P, _I, _I, _P, _P, _F, _F]),
     "ncb_logits_temperature": (_I, [_P, _P, _I, _I, _F]),

@@ -211,6 +211,61 @@ class CudaTokenSampler:
         return int(n.value)
 
 
+def dtype_code(dtype) -> int:
+    """NCB_DTYPE_* of a torch dtype; ValueError for one the library does not take."""
+    import torch
+    code = {torch.float32: native.DTYPE_F32, torch.float16: native.DTYPE_F16,
+            torch.bfloat16: native.DTYPE_BF16}.get(dtype)
+    if code is None:
+        raise ValueError(f"values of type {dtype}: float32, float16 or bfloat16 needed")
+    return code
+
+
+def sample_rows_min_p_device(logits, uniforms, tokens, temperature=None, top_k=None, top_p=None,
+                             min_p=None, logprobs=None, kept=None, flags=None,
+                             stream=None) -> None:
+    """One token per row of `logits` ([rows, vocab] float32, float16 or bfloat16 on a GPU, any row
+    stride), every row with options of its own: ncb_sample_rows_min_p_device in
+    include/navsampler.h states the arithmetic. `uniforms`, `temperature`, `top_p`, `min_p`,
+    `logprobs` are float32, `top_k`, `tokens`, `kept`, `flags` 32-bit integers, each `rows`
+    contiguous values on the logits' device; an option that is None is off in every row
+    (temperature: 1). Asynchronous on `stream` (None: the legacy default stream, as in the
+    other calls); it runs on the logits' device and needs no sampler."""
+    if logits.dim() != 2:
+        raise ValueError("logits must be [rows, vocab]")
+    rows, vocab = logits.shape
+    device = logits.device
+    if device.type != "cuda":
+        raise ValueError("logits must be on a CUDA device")
+    if vocab > 1 and logits.stride(1) != 1:
+        raise ValueError("a row's logits must be contiguous")
+    ptrs = []
+    for name, t, kind in (("uniforms", uniforms, _F32), ("temperature", temperature, _F32),
+                          ("top_k", top_k, _I32), ("top_p", top_p, _F32), ("min_p", min_p, _F32),
+                          ("tokens", tokens, _I32), ("logprobs", logprobs, _F32),
+                          ("kept", kept, _I32), ("flags", flags, _I32)):
+        if t is None:
+            ptrs.append(None)
+            continue
+        if str(t.dtype) not in kind or t.numel() != rows or not t.is_contiguous() \
+                or t.device != device:
+            raise ValueError(f"{name} must be {rows} contiguous values of {' or '.join(kind)} "
+                             f"on {device}")
+        ptrs.append(t.data_ptr())
+    if uniforms is None or tokens is None:
+        raise ValueError("uniforms and tokens are needed")
+    import torch
+    ld = logits.stride(0) if rows > 1 else vocab
+    with torch.cuda.device(device):
+        st = load().ncb_sample_rows_min_p_device(logits.data_ptr(), dtype_code(logits.dtype), rows,
+                                                 vocab, ld, *ptrs, _stream_ptr(stream))
+    check(st, "ncb_sample_rows_min_p_device")
+
+
+_F32 = ("torch.float32",)
+_I32 = ("torch.int32", "torch.uint32")
+
+
 def fast_exp_max_steps(x_lo: float, x_hi: float) -> int:
     """Largest float-step distance between the bucketed kernel's fast exp
     estimate and the correctly rounded exp over every float in [x_lo, x_hi]."""
@@ -220,4 +275,5 @@ def fast_exp_max_steps(x_lo: float, x_hi: float) -> int:
     return int(out.value)
 
 
-__all__ = ["CudaTokenSampler", "NcbSamplerParams", "make_params", "native", "fast_exp_max_steps"]
+__all__ = ["CudaTokenSampler", "NcbSamplerParams", "make_params", "native", "fast_exp_max_steps",
+           "sample_rows_min_p_device", "dtype_code"]

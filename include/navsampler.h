@@ -364,6 +364,54 @@ NCB_API int ncb_sample_rows_min_p_device(const void* d_logits, int dtype, int ro
                                          int32_t* d_tokens, float* d_logprobs, int32_t* d_kept,
                                          uint32_t* d_flags, void* stream);
 
+/* ---- LM head with low-rank adapters of many requests -------------------------
+ * The projection that gives the samplers their logits
+ * (ModernDecoderModel.ComputeLogits, Neuraval/Models/ModernDecoderModel.cs:221-240;
+ * LoRA weights, Neuraval/Peft), for a batch whose rows belong to requests with
+ * adapters of their own:
+ *   out[n, :] = W x_n + scale_s * B_s (A_s x_n),  s = adapter_ids[n]
+ * W is [out_features, in_features], A_s [rank_s, in_features], B_s
+ * [out_features, rank_s], x [rows, in_features], all of the handle's dtype
+ * (NCB_DTYPE_F16 or NCB_DTYPE_BF16). Products are summed in fp32 and rounded
+ * once, to the output's type. No sum's order depends on timing: the same call
+ * gives the same bits.
+ *
+ * The handle owns packed copies of the adapters and its scratch; like a
+ * sampler it is single-stream: calls on one handle must not overlap on the GPU
+ * (graphs captured from one handle share its scratch and may not run at the
+ * same time; use a handle each). Everything is stream-ordered. */
+typedef struct NcbAdapterHead NcbAdapterHead;
+
+/* max_rows rows per call at most, adapter slots 0 .. max_adapters-1 (<= 1024),
+ * ranks up to max_rank (<= 128; max_adapters and max_rank may be 0: no
+ * adapters). Allocates the slots and the scratch. */
+NCB_API int ncb_adapter_head_create(int device, int dtype, int in_features, int out_features,
+                                    int max_rows, int max_adapters, int max_rank,
+                                    NcbAdapterHead** out);
+/* Waits for the device before it frees. */
+NCB_API int ncb_adapter_head_destroy(NcbAdapterHead* head);
+/* The shared weight, rows `ld` elements apart. It is read in place by later
+ * calls and has to stay allocated, except where its base or row stride is not a
+ * multiple of 16 bytes: then this call copies it (and allocates the copy, so
+ * not while a stream is captured). Call it again after changing the weight. */
+NCB_API int ncb_adapter_head_set_weight_device(NcbAdapterHead* head, const void* d_weight,
+                                               int64_t ld, void* stream);
+/* Copies adapter `slot` in (1 <= rank <= max_rank, finite scale): d_a
+ * [rank, in_features], rows lda apart; d_b [out_features, rank], rows ldb apart. */
+NCB_API int ncb_adapter_head_set_adapter_device(NcbAdapterHead* head, int slot, const void* d_a,
+                                                int64_t lda, const void* d_b, int64_t ldb,
+                                                int rank, float scale, void* stream);
+/* Empties a slot: its rows get the shared projection alone. */
+NCB_API int ncb_adapter_head_clear_adapter_device(NcbAdapterHead* head, int slot, void* stream);
+/* d_x [rows, in_features] of the handle's dtype, rows ldx apart; d_adapter_ids
+ * rows int32 slots, or NULL for none (an id outside the slots, -1 say, or of an
+ * empty slot takes the shared projection alone); d_out [rows, out_features] of
+ * out_dtype (NCB_DTYPE_F32 or the handle's), rows ldo apart; values between
+ * rows are left as they were. rows = 0 is a no-op. */
+NCB_API int ncb_adapter_head_project_device(NcbAdapterHead* head, const void* d_x, int64_t ldx,
+                                            int rows, const int32_t* d_adapter_ids, void* d_out,
+                                            int out_dtype, int64_t ldo, void* stream);
+
 /* ---- diagnostics ----------------------------------------------------------
  * Rows this handle has redone on the exact full-sort kernel since it was
  * created: top-k rows whose ties overflowed the candidate buffers, and

@@ -28,6 +28,7 @@ UNITS = {
     "softmax_rows.cu": [],
     # 64-bit sums decide; contraction only makes them more exact
     "sample_min_p.cu": [],
+    "adapter_head.cu": [],
 }
 def nvcc() -> str:
     cand = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "bin", "nvcc")

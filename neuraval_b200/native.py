@@ -92,6 +92,12 @@ SIGNATURES = {
     "ncb_softmax_rows_device": (_I, [_P, _P, _I, _I, _P]),
     "ncb_sample_rows_min_p_device": (_I, [_P, _I, _I, _I, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P,
                                           _P]),
+    "ncb_adapter_head_create": (_I, [_I, _I, _I, _I, _I, _I, _I, ctypes.POINTER(_P)]),
+    "ncb_adapter_head_destroy": (_I, [_P]),
+    "ncb_adapter_head_set_weight_device": (_I, [_P, _P, _L, _P]),
+    "ncb_adapter_head_set_adapter_device": (_I, [_P, _I, _P, _L, _P, _L, _I, _F, _P]),
+    "ncb_adapter_head_clear_adapter_device": (_I, [_P, _I, _P]),
+    "ncb_adapter_head_project_device": (_I, [_P, _P, _L, _I, _P, _P, _I, _L, _P]),
     "ncb_logits_repetition_penalty": (_I, [_P, _P, _I, _I, _P, _P, _F]),
     "ncb_logits_frequency_presence_penalty": (_I, [_P, _P, _I, _I, _P, _P, _F, _F]),
     "ncb_logits_temperature": (_I, [_P, _P, _I, _I, _F]),

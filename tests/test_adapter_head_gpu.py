@@ -131,7 +131,8 @@ def test_random_values(shape, dtype, out):
 
 
 @pytest.mark.parametrize("ranks,rows", [([128], 40), ([64, 3], 20), ([16] * 40, 40), ([5] * 300, 300),
-                                        ([1, 128, 2, 127, 15, 16, 17], 64)], ids=str)
+                                        ([1, 128, 2, 127, 15, 16, 17], 64)],
+                         ids=["128", "64_3", "16x40", "5x300", "mixed"])
 def test_ranks_and_many_adapters(ranks, rows):
     """One adapter for all rows, an adapter for each row, ranks on both sides of 16."""
     rng = np.random.default_rng(len(ranks))
@@ -223,8 +224,8 @@ def test_weight_set_again():
 
 
 def test_non_finite_rows_stay_alone():
-    """A row of x with NaN, or whose adapter's A overflows, leaves the other rows alone."""
-    import torch
+    """A row of x with NaN, an adapter with NaN in A or an infinity in B: NaN in the rows that use
+    it, and the other rows as they are."""
     c = Case(20, 128, 260, [16, 16], np.arange(20) % 2, "bf16", 15, whole=True)
     want = c.want()[0].float()
     c.x[3, 5] = float("nan")
@@ -233,6 +234,14 @@ def test_non_finite_rows_stay_alone():
     assert got[3].isnan().all()
     keep = [i for i in range(20) if i != 3]
     assert (got[keep] == want[keep]).all()
+    for spoil in (lambda: c.a[1].view(-1)[70:71].fill_(float("nan")), lambda: c.b[1].view(-1)[999:1000].fill_(float("inf"))):
+        c = Case(20, 128, 260, [16, 16], np.arange(20) % 2, "bf16", 15, whole=True)
+        spoil()
+        with c.head() as h:
+            got = c.run(h)
+            assert got[1::2].isnan().all() and (got[::2] == want[::2]).all()
+            h.set_adapter(1, c.a[0], c.b[0], 1.0)  # a sound one in its place
+            assert c.run(h).isfinite().all()
 
 
 def test_refusals_with_a_head():

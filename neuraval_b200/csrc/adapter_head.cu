@@ -47,38 +47,50 @@ constexpr int AH_NT = 256;        // rows of the batch per tile at most
 constexpr int AH_A_BYTES = AH_BM * AH_BK * 2;
 constexpr int AH_MAX_STAGES = 12;
 constexpr int AH_SMEM = 208 * 1024;  // stages; leaves room for a shrink CTA on the SM
-constexpr int AH_THREADS = 192;   // four epilogue warps, a copying and a multiplying one
+constexpr int AH_EPILOGUE = 8;    // warps that write results
+constexpr int AH_THREADS = (AH_EPILOGUE + 2) * 32;  // and a copying and a multiplying one
+constexpr int AH_PIECE = 8;       // stages added up in TMEM for an fp32 output
 constexpr int AH_PAIR = 2;        // adapter entries per stage
 
 struct AhArgs {
   const void* x;
   int64_t ldx;
   int rows, in, kpad, out, slots, slices;  // slices: entries a slot can have
-  int nt, tiles_n;                         // rows per tile, tiles of rows
+  int nt, nh, tiles_n;                     // rows per tile, of it per CTA, tiles of rows
   const int32_t* ids;
   const void* a;        // [slots][16 slices][kpad]
   const int32_t* ranks; // per slot; 0: empty, < 0: |rank|, and B holds a non-finite value
   const float* scales;
-  void* u;              // [tiles_n][max_entries][2][nt][16]
+  void* u;              // [tiles_n][max_entries][nt / nh][hi, lo][nh][16]
   int32_t* entries;     // [tiles_n][max_entries] slot * slices + slice
   int32_t* counts;      // [tiles_n]
-  int max_entries;
+  int max_entries, opad;
   void* y;
   int64_t ldo;
+  int share;  // outputs per CTA
   uint32_t idesc;
   int stages;
   uint32_t* error_word;
 };
 
 // ---- loading a slot ---------------------------------------------------------------
-// B goes to [slice][out][16]: a 128-row tile of an entry is 4 KiB in a row. A
+// Where value j of row r lies in a [rows][16] matrix as the tensor cores read it
+// from shared memory (rows of 32 bytes, their halves swapped in every other group
+// of four rows). B and U are kept like this in global memory, so that a tile of
+// them is contiguous and is copied by rows of 512 bytes: TMA boxes of 32-byte rows
+// took five times as long.
+__host__ __device__ __forceinline__ int64_t ah_at(int64_t r, int j) {
+  return r * 16 + (j ^ ((int)(r >> 2) & 1) << 3);
+}
+
+// B goes to [slice][outputs][16]: a 128-row tile of an entry is 4 KiB in a row. A
 // value of B that is not finite would reach every row of a tile (0 times NaN);
 // it is stored as 0 and the slot marked, and the slot's own rows come out as NaN.
 template <typename E>
 __global__ void adapter_pack_kernel(E* a, E* b, int32_t* ranks, float* scales, int slot, int in,
-                                    int kpad, int out, int slices, const E* sa, int64_t lda,
-                                    const E* sb, int64_t ldb, int rank) {
-  const int64_t na = (int64_t)slices * 16 * kpad, nb = (int64_t)slices * out * 16;
+                                    int kpad, int out, int opad, int slices, const E* sa,
+                                    int64_t lda, const E* sb, int64_t ldb, int rank) {
+  const int64_t na = (int64_t)slices * 16 * kpad, nb = (int64_t)slices * opad * 16;
   const int64_t t0 = blockIdx.x * (int64_t)blockDim.x + threadIdx.x, dt = (int64_t)gridDim.x * blockDim.x;
   for (int64_t i = t0; i < na; i += dt) {
     const int64_t j = i / kpad, k = i % kpad;
@@ -86,13 +98,13 @@ __global__ void adapter_pack_kernel(E* a, E* b, int32_t* ranks, float* scales, i
   }
   bool bad = false;
   for (int64_t i = t0; i < nb; i += dt) {
-    const int64_t j = i / ((int64_t)out * 16) * 16 + i % 16, v = i / 16 % out;
-    E x = j < rank ? sb[v * ldb + j] : E(0.0f);
+    const int64_t slice = i / ((int64_t)opad * 16), j = slice * 16 + i % 16, v = i / 16 % opad;
+    E x = j < rank && v < out ? sb[v * ldb + j] : E(0.0f);
     if (!(fabsf((float)x) < INFINITY)) {
       bad = true;
       x = E(0.0f);
     }
-    b[slot * nb + i] = x;
+    b[slot * nb + slice * opad * 16 + ah_at(v, (int)(i % 16))] = x;
   }
   if (bad) ranks[slot] = -rank;
 }
@@ -110,26 +122,20 @@ __global__ void adapter_align_kernel(E* to, int64_t pitch, const E* from, int64_
 }
 
 // ---- u = scale A x --------------------------------------------------------------------
-template <typename E>
-__device__ __forceinline__ void ah_mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  if constexpr (std::is_same_v<E, __nv_bfloat16>)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
 constexpr int AS_THREADS = 256;
+static_assert(AS_THREADS >= AH_NT && AS_THREADS * 4 >= AH_MAX_ADAPTERS, "a row, four slots per thread");
 
+template <typename E>
+__device__ __forceinline__ float2 ah_pair(uint32_t w) {
+  if constexpr (std::is_same_v<E, __nv_bfloat16>)
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+  else
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
 // Eight values of a row of x from column k on; columns past the row are 0.
 template <typename E>
 __device__ __forceinline__ uint4 ah_row8(const E* row, int k, int in) {
-  if (k + 8 <= in) return *reinterpret_cast<const uint4*>(row + k);
+  if (k + 8 <= in) return __ldg(reinterpret_cast<const uint4*>(row + k));
   uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int i = 0; i < 8; ++i)
@@ -138,37 +144,76 @@ __device__ __forceinline__ uint4 ah_row8(const E* row, int k, int in) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// grid (CTAs, tiles_n). Every CTA lists its tile's entries; the work is dealt out
-// as (entry, 16 rows): one 16 x 16 product over the inner axis, eight warps taking
-// every eighth 32 columns and their sums added in the order of the warps. It only
-// delays the head's last steps, which are the ones that wait for it.
+// grid (nt, tiles_n, slices): a CTA for 16 ranks of a row's slot, 8 columns per
+// thread and turn, summed over the threads at the end. Every CTA that has
+// something to write lists its tile's entries for itself (the order of the slots)
+// while its loads are under way. The operations are few (rows * rank * in); what
+// counts is that the kernel ends while the head still multiplies its first tile,
+// so it is spread over as many CTAs as there are rows, and leaves the SM room for
+// the head beside it.
 template <typename E>
-__global__ void __launch_bounds__(AS_THREADS) adapter_shrink_kernel(const AhArgs g) {
+__global__ void __launch_bounds__(AS_THREADS, 2) adapter_shrink_kernel(const AhArgs g) {
   asm volatile("griddepcontrol.launch_dependents;");
-  __shared__ uint32_t named[AH_MAX_ADAPTERS / 32];
-  __shared__ int32_t ids[AH_NT];
+  __shared__ uint32_t taken[AH_MAX_ADAPTERS / 4];  // a byte per slot: its entries, once named
+  __shared__ int32_t first[AH_MAX_ADAPTERS];       // and the first of them
   __shared__ int32_t warp_sum[AS_THREADS / 32];
-  __shared__ float part[AS_THREADS / 32][16][17];
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, tile = blockIdx.y;
-  const int n0 = tile * g.nt;
-  int32_t* entries = g.entries + (int64_t)tile * g.max_entries;
-  if (t < AH_MAX_ADAPTERS / 32) named[t] = 0;
-  __syncthreads();
-  if (t < g.nt) {
-    int s = n0 + t < g.rows ? g.ids[n0 + t] : -1;
-    if (s < 0 || s >= g.slots || g.ranks[s] == 0) s = -1;
-    ids[t] = s;
-    if (s >= 0) atomicOr(&named[s >> 5], 1u << (s & 31));
-  }
-  __syncthreads();
-  // entries in the order of the slots, four slots per thread
-  int mine[4], sum = 0;
+  __shared__ float part[AS_THREADS / 32][16];
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int r = blockIdx.x, tile = blockIdx.y, slice = blockIdx.z, n0 = tile * g.nt;
+  taken[t] = 0;
+  auto slot_of = [&](int row) {
+    const int s = row < g.rows ? g.ids[row] : -1;
+    return s >= 0 && s < g.slots ? s : -1;
+  };
+  const int slot = slot_of(n0 + r), other = t < g.nt ? slot_of(n0 + t) : -1;
+  const int rank = slot >= 0 ? g.ranks[slot] : 0;
+  const int mine = (abs(rank) + 15) / 16;
+  if (slice > 0 && slice >= mine) return;
+  const int used = other >= 0 ? (abs(g.ranks[other]) + 15) / 16 : 0;
+
+  float acc[16] = {};
+  if (mine) {
+    const E* a = static_cast<const E*>(g.a) + ((int64_t)slot * g.slices + slice) * 16 * (int64_t)g.kpad;
+    const E* x = static_cast<const E*>(g.x) + (int64_t)(n0 + r) * g.ldx;
+    for (int k = t * 8; k < g.kpad; k += AS_THREADS * 8) {
+      const uint4 xv = ah_row8(x, k, g.in);
+      uint4 av[16];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int s = 4 * t + j;
-    mine[j] = named[s >> 5] >> (s & 31) & 1 ? (abs(g.ranks[s]) + 15) / 16 : 0;
-    sum += mine[j];
+      for (int j = 0; j < 16; ++j)
+        av[j] = __ldg(reinterpret_cast<const uint4*>(a + (int64_t)j * g.kpad + k));
+      const float2 x0 = ah_pair<E>(xv.x), x1 = ah_pair<E>(xv.y), x2 = ah_pair<E>(xv.z),
+                   x3 = ah_pair<E>(xv.w);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float2 a0 = ah_pair<E>(av[j].x), a1 = ah_pair<E>(av[j].y), a2 = ah_pair<E>(av[j].z),
+                     a3 = ah_pair<E>(av[j].w);
+        acc[j] = fmaf(a0.x, x0.x, fmaf(a0.y, x0.y, acc[j]));
+        acc[j] = fmaf(a1.x, x1.x, fmaf(a1.y, x1.y, acc[j]));
+        acc[j] = fmaf(a2.x, x2.x, fmaf(a2.y, x2.y, acc[j]));
+        acc[j] = fmaf(a3.x, x3.x, fmaf(a3.y, x3.y, acc[j]));
+      }
+    }
   }
+  // sums over the warp: lane l ends with those of rank l / 2
+#pragma unroll
+  for (int half = 8, o = 16; half > 0; half >>= 1, o >>= 1) {
+    const bool upper = lane & o;
+#pragma unroll
+    for (int j = 0; j < half; ++j) {
+      const float send = upper ? acc[j] : acc[j + half], keep = upper ? acc[j + half] : acc[j];
+      acc[j] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+    }
+  }
+  acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], 1);
+  if ((lane & 1) == 0) part[warp][lane >> 1] = acc[0];
+
+  // ---- the tile's entries -------------------------------------------------------------
+  __syncthreads();
+  if (used) reinterpret_cast<uint8_t*>(taken)[other] = (uint8_t)used;  // equal for equal slots
+  __syncthreads();
+  const uint32_t four = taken[t];
+  const int c0 = four & 255, c1 = four >> 8 & 255, c2 = four >> 16 & 255, c3 = four >> 24;
+  const int sum = c0 + c1 + c2 + c3;
   int inc = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -183,74 +228,40 @@ __global__ void __launch_bounds__(AS_THREADS) adapter_shrink_kernel(const AhArgs
     if (w < warp) at += warp_sum[w];
     count += warp_sum[w];
   }
-  if (blockIdx.x == 0 && t == 0) g.counts[tile] = count;
-  const int blocks = g.nt / 16;
-  for (int first = 0; first < count * blocks; first += gridDim.x) {
-    const int item = first + blockIdx.x;
-    // the thread whose slots hold the item's entry says which it is
-    __shared__ int32_t s_slot, s_slice;
-    __syncthreads();
-    if (item < count * blocks) {
-      const int e = item / blocks;
-      int b = at;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (e >= b && e < b + mine[j]) {
-          s_slot = 4 * t + j;
-          s_slice = e - b;
-        }
-        b += mine[j];
-      }
+  first[4 * t] = at;
+  first[4 * t + 1] = at + c0;
+  first[4 * t + 2] = at + c0 + c1;
+  first[4 * t + 3] = at + c0 + c1 + c2;
+  if (r == 0 && slice == 0) {  // row 0's CTA writes the list down
+    int32_t* entries = g.entries + (int64_t)tile * g.max_entries;
+    for (int j = 0, e = at; j < 4; ++j)
+      for (int i = 0; i < (int)(four >> (8 * j) & 255); ++i) entries[e++] = (4 * t + j) * g.slices + i;
+    if (t == 0) g.counts[tile] = count;
+  }
+  __syncthreads();
+
+  // ---- this row of every entry's U ------------------------------------------------------
+  E* u = static_cast<E*>(g.u) +
+         ((int64_t)tile * g.max_entries * 2 * g.nt + r / g.nh * 2 * g.nh) * 16;
+  const int own = mine ? first[slot] : 0, row = r % g.nh;
+  if (slice == 0)
+    for (int i = t; i < 4 * count; i += AS_THREADS) {  // zeros, 16 bytes at a time
+      const int e = i >> 2;
+      if (e >= own && e < own + mine) continue;
+      *reinterpret_cast<uint4*>(u + (int64_t)e * 2 * g.nt * 16 + (i & 2 ? g.nh * 16 : 0) + row * 16 +
+                                (i & 1) * 8) = make_uint4(0, 0, 0, 0);
     }
-    __syncthreads();
-    if (item >= count * blocks) continue;
-    const int e = item / blocks, r0 = item % blocks * 16;
-    const int slot = s_slot, slice = s_slice;
-    if (r0 == 0 && t == 0) entries[e] = slot * g.slices + slice;
-    const bool any = __syncthreads_or(t < 16 && ids[r0 + t] == slot);
-    float u = 0.0f;
-    if (any) {
-      const E* a = static_cast<const E*>(g.a) +
-                   ((int64_t)slot * g.slices + slice) * 16 * (int64_t)g.kpad;
-      const int q = lane >> 2, c = (lane & 3) * 8;
-      const int na = n0 + r0 + q, nb = na + 8;
-      const E* x = static_cast<const E*>(g.x);
-      const E* xa = x + (int64_t)min(na, g.rows - 1) * g.ldx;
-      const E* xb = x + (int64_t)min(nb, g.rows - 1) * g.ldx;
-      const E* pa = a + (int64_t)q * g.kpad;
-      const E* pb = a + (int64_t)(q + 8) * g.kpad;
-      float acc[2][4] = {};
-      // A lane's eight values of a row feed two products: the inner axis may be
-      // permuted as long as both operands are.
-#pragma unroll 4
-      for (int k = warp * 32 + c; k < g.kpad; k += AS_THREADS) {
-        const uint4 va = ah_row8(xa, k, g.in), vb = ah_row8(xb, k, g.in);
-        const uint4 wa = *reinterpret_cast<const uint4*>(pa + k);
-        const uint4 wb = *reinterpret_cast<const uint4*>(pb + k);
-        const uint32_t f0[4] = {va.x, vb.x, va.y, vb.y}, f1[4] = {va.z, vb.z, va.w, vb.w};
-        ah_mma<E>(acc[0], f0, wa.x, wa.y);
-        ah_mma<E>(acc[1], f0, wb.x, wb.y);
-        ah_mma<E>(acc[0], f1, wa.z, wa.w);
-        ah_mma<E>(acc[1], f1, wb.z, wb.w);
-      }
+  if (mine && t < 16) {
+    float v = 0.0f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          part[warp][q + 8 * (i >> 1)][8 * h + 2 * (lane & 3) + (i & 1)] = acc[h][i];
-      __syncthreads();
-      if (ids[r0 + t / 16] == slot) {
-        for (int w = 0; w < AS_THREADS / 32; ++w) u += part[w][t / 16][t % 16];
-        u *= g.scales[slot];
-        if (g.ranks[slot] < 0) u = NAN;
-      }
-    }
-    const E hi = E(u);
-    const E lo = E(fabsf((float)hi) < INFINITY ? u - (float)hi : 0.0f);
-    E* to = static_cast<E*>(g.u) +
-            (((int64_t)tile * g.max_entries + e) * 2 * g.nt + r0) * 16 + t;
+    for (int w = 0; w < AS_THREADS / 32; ++w) v += part[w][t];
+    v *= g.scales[slot];
+    if (rank < 0) v = NAN;
+    const E hi = E(v);
+    const E lo = E(fabsf((float)hi) < INFINITY ? v - (float)hi : 0.0f);
+    E* to = u + (int64_t)(own + slice) * 2 * g.nt * 16 + ah_at(row, t);
     to[0] = hi;
-    to[(int64_t)g.nt * 16] = lo;
+    to[(int64_t)g.nh * 16] = lo;
   }
 }
 
@@ -284,24 +295,35 @@ __device__ __forceinline__ void ah_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
                : "memory");
 }
-__device__ __forceinline__ void ah_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+// Shared addresses of a pair's CTAs differ in bit 24: without it, the first one's.
+constexpr uint32_t AH_FIRST = 0xFEFFFFFFu;
+template <int CG>
+__device__ __forceinline__ void ah_arrive_first(uint32_t bar) {
+  if constexpr (CG == 1)
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+  else
+    asm volatile(
+        "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, 0;\n"
+        " mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n}" ::"r"(bar)
+        : "memory");
 }
-__device__ __forceinline__ void ah_copy2(uint32_t to, const CUtensorMap* map, uint32_t bar, int x,
+// Copies into this CTA's own shared memory; in a pair the first CTA's barrier
+// counts the bytes of both.
+template <int CG>
+__device__ __forceinline__ void ah_copy(uint32_t to, const CUtensorMap* map, uint32_t bar, int x,
                                          int y) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
-          to),
-      "l"(map), "r"(bar), "r"(x), "r"(y)
-      : "memory");
-}
-__device__ __forceinline__ void ah_copy3(uint32_t to, const CUtensorMap* map, uint32_t bar, int x,
-                                         int y, int z) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::
-          "r"(to),
-      "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
-      : "memory");
+  if constexpr (CG == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::
+            "r"(to),
+        "l"(map), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::
+            "r"(to),
+        "l"(map), "r"(bar & AH_FIRST), "r"(x), "r"(y)
+        : "memory");
 }
 // Shared-memory operand whose rows of `span` bytes (32 or 128) lie one behind the
 // other in the TMA's swizzle of that span, eight rows to a group.
@@ -309,45 +331,102 @@ __device__ __forceinline__ uint64_t ah_operand(uint32_t addr, int span) {
   return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)1 << 16 | (uint64_t)(span * 8 >> 4) << 32 |
          (uint64_t)1 << 46 | (uint64_t)(span == 128 ? 2 : 6) << 61;
 }
+template <int CG>
 __device__ __forceinline__ void ah_multiply(uint32_t acc, uint64_t a, uint64_t b, uint32_t idesc,
                                             bool add) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(acc),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
-      : "memory");
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(acc),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(acc),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
 }
+// The barrier (of both CTAs of a pair) is arrived at when the products issued so
+// far have ended.
+template <int CG>
 __device__ __forceinline__ void ah_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-               : "memory");
+  if constexpr (CG == 1)
+    asm volatile(
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::
+            "r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void ah_all_sync() {
+  if constexpr (CG == 1) {
+    __syncthreads();
+  } else {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
 }
 
-template <typename O>
-__device__ __forceinline__ O ah_out(uint32_t bits) {
-  return O(__uint_as_float(bits));
+__device__ __forceinline__ void ah_load16(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
-template <typename O>
+// One CTA per SM, or (CG = 2) a pair of CTAs on two SMs whose tensor cores work on
+// one product: each holds its own 128 outputs and half of the rows of x, and reads
+// the other half from its neighbour.
+//
+// The outputs are dealt out evenly: every CTA takes g.share of them, a multiple of
+// 16, in tiles of 128 and a last, lower one, so that all read the same number of
+// weight bytes (whole tiles would leave a sixth of the SMs idle at 250 tiles).
+//
+// CPT > 0 (fp32 output): the sum over the inner axis is cut into pieces of
+// AH_PIECE stages, each summed in TMEM from zero and added up in registers, CPT
+// columns of the batch per thread. The tensor cores truncate their sums, an error
+// that grows with the number of additions: 256 in a row (4096 values) measured
+// 3.9e-6 of the result, eight pieces of 32 a sixth of that. A 16-bit output's own
+// rounding hides it, so there the sum is one piece.
+template <typename O, int CG, int CPT>
 __global__ void __launch_bounds__(AH_THREADS, 1)
-    head_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
-                const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_u,
-                const AhArgs g) {
+    head_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_low,
+                const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_b,
+                const __grid_constant__ CUtensorMap map_u, const AhArgs g) {
   extern __shared__ uint8_t ah_raw[];
   __shared__ uint64_t bars[2 * AH_MAX_STAGES + 4];
   __shared__ uint32_t s_tmem;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int rank = CG == 1 ? 0 : (int)(blockIdx.x & 1);  // in the pair
   const uint32_t stage0 = (ah_smem(ah_raw) + 1023) & ~1023u;
-  const uint32_t stage_bytes = AH_A_BYTES + g.nt * 128;
+  const int nh = g.nh;  // rows of x in this CTA
+  const uint32_t stage_bytes = AH_A_BYTES + nh * 128;
   const uint32_t full = ah_smem(bars), empty = full + 8 * AH_MAX_STAGES,
                  done = empty + 8 * AH_MAX_STAGES, drained = done + 16;
   uint32_t columns = 32;
   while (columns < 2u * g.nt) columns *= 2;
-  if (warp == 5) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     ah_smem(&s_tmem)),
-                 "r"(columns)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  if (warp == AH_EPILOGUE + 1) {
+    if constexpr (CG == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                       ah_smem(&s_tmem)),
+                   "r"(columns)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                       ah_smem(&s_tmem)),
+                   "r"(columns)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
   }
   if (t == 0) {
     for (int i = 0; i < AH_MAX_STAGES; ++i) {
@@ -356,156 +435,212 @@ __global__ void __launch_bounds__(AH_THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(done + 8 * i) : "memory");
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 128;" ::"r"(drained + 8 * i) : "memory");
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(drained + 8 * i),
+                   "r"(AH_EPILOGUE * CG)
+                   : "memory");
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  ah_all_sync<CG>();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = s_tmem;
-  const int tiles_m = (g.out + AH_BM - 1) / AH_BM, tiles = tiles_m * g.tiles_n;
   const int steps = (g.in + AH_BK - 1) / AH_BK;
+  const int piece = CPT ? AH_PIECE : steps;  // stages added up in TMEM
+  const int pieces = (steps + piece - 1) / piece;
+  const int v_begin = blockIdx.x * g.share, tiles_m = (g.share + AH_BM - 1) / AH_BM;
 
-  if (warp == 4) {
-    if (lane == 0) {  // ---- copies -----------------------------------------------------
-      int s = 0;
-      uint32_t phase = 0;
-      int issued = 0;
-      bool ok = true, waited = false;
-      for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
-        const int m = tile / g.tiles_n, n = tile % g.tiles_n;
-        for (int k = 0; k < steps; ++k) {
-          if (!(ok = ah_wait(empty + 8 * s, phase ^ 1))) break;
+  if (warp == AH_EPILOGUE) {  // ---- copies: the warp waits together, a lane issues ------------
+    int s = 0, issued = 0;
+    uint32_t phase = 0;
+    bool ok = true, waited = false;
+    for (int i = 0; ok && i < tiles_m * g.tiles_n; ++i) {
+      const int m = i / g.tiles_n, n = i % g.tiles_n;
+      const int v0 = v_begin + m * AH_BM, high = min(AH_BM, g.share - m * AH_BM);
+      const int32_t* entries = g.entries + (int64_t)n * g.max_entries;
+      int count = 0, mine = 0;  // entries of the tile of rows; lane l holds the l-th of 32
+      if (waited && g.ids) {
+        count = __ldcg(g.counts + n);
+        if (lane < count) mine = __ldcg(entries + lane);
+      }
+      for (int k = 0; k < steps; ++k) {
+        if (!(ok = ah_wait(empty + 8 * s, phase ^ 1))) break;
+        if (lane == 0) {
           const uint32_t a = stage0 + s * stage_bytes, bar = full + 8 * s;
-          ah_expect(bar, stage_bytes);
-          ah_copy2(a, &map_w, bar, k * AH_BK, m * AH_BM);
-          ah_copy2(a + AH_A_BYTES, &map_x, bar, k * AH_BK, n * g.nt);
-          ++issued;
-          if (++s == g.stages) s = 0, phase ^= 1;
+          if (rank == 0) ah_expect(bar, CG * (high * 128 + nh * 128));
+          ah_copy<CG>(a, high == AH_BM ? &map_w : &map_low, bar, k * AH_BK, v0);
+          ah_copy<CG>(a + AH_A_BYTES, &map_x, bar, k * AH_BK, n * g.nt + rank * nh);
         }
-        if (!ok) break;
-        if (!waited) {  // what follows reads the shrink kernel's results
-          asm volatile("griddepcontrol.wait;" ::: "memory");
-          asm volatile("fence.proxy.async.global;" ::: "memory");
-          waited = true;
+        __syncwarp();
+        ++issued;
+        if (++s == g.stages) s = 0, phase ^= 1;
+      }
+      if (!ok) break;
+      if (!waited) {  // what follows reads the shrink kernel's results
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        asm volatile("fence.proxy.async.global;" ::: "memory");
+        waited = true;
+        if (g.ids) {
+          count = __ldcg(g.counts + n);
+          if (lane < count) mine = __ldcg(entries + lane);
         }
-        const int count = g.ids ? *(volatile const int32_t*)(g.counts + n) : 0;
-        for (int e = 0; e < count; e += AH_PAIR) {
-          if (!(ok = ah_wait(empty + 8 * s, phase ^ 1))) break;
-          const int both = count - e < AH_PAIR ? count - e : AH_PAIR;
+      }
+      for (int e = 0; e < count; e += AH_PAIR) {
+        if (e && (e & 31) == 0) mine = e + lane < count ? __ldcg(entries + e + lane) : 0;
+        if (!(ok = ah_wait(empty + 8 * s, phase ^ 1))) break;
+        const int both = min(AH_PAIR, count - e);
+        const int z0 = __shfl_sync(0xffffffffu, mine, e & 31),
+                  z1 = __shfl_sync(0xffffffffu, mine, (e & 31) + 1);
+        if (lane == 0) {
           const uint32_t a = stage0 + s * stage_bytes, bar = full + 8 * s;
-          ah_expect(bar, both * (AH_BM * 32 + 2 * g.nt * 32));
+          if (rank == 0) ah_expect(bar, CG * both * (AH_BM * 32 + 2 * nh * 32));
           for (int j = 0; j < both; ++j) {
-            ah_copy3(a + j * AH_BM * 32, &map_b, bar, 0, m * AH_BM,
-                     *(volatile const int32_t*)(g.entries + (int64_t)n * g.max_entries + e + j));
-            const int row = (n * g.max_entries + e + j) * 2 * g.nt;
-            ah_copy2(a + AH_A_BYTES + j * g.nt * 64, &map_u, bar, 0, row);
-            ah_copy2(a + AH_A_BYTES + j * g.nt * 64 + g.nt * 32, &map_u, bar, 0, row + g.nt);
+            ah_copy<CG>(a + j * AH_BM * 32, &map_b, bar, 0, (int)(((int64_t)(j ? z1 : z0) * g.opad + v0) / 16));
+            ah_copy<CG>(a + AH_A_BYTES + j * nh * 64, &map_u, bar, 0,
+                         ((n * g.max_entries + e + j) * 2 * g.nt + rank * 2 * nh) / 16);
           }
-          ++issued;
-          if (++s == g.stages) s = 0, phase ^= 1;
         }
+        __syncwarp();
+        ++issued;
+        if (++s == g.stages) s = 0, phase ^= 1;
       }
-      if (!ok) {  // gave up: no copy may be in flight when the CTA ends
-        atomicOr(g.error_word, 1u);
-        for (int i = 0; i < g.stages && i < issued; ++i) {
-          if (s-- == 0) s = g.stages - 1, phase ^= 1;
-          ah_wait(full + 8 * s, phase);
-        }
-      }
-      if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
     }
-  } else if (warp == 5) {
-    if (lane == 0) {  // ---- products -----------------------------------------------------
+    if (!ok) {  // gave up: no copy may be in flight when the CTA ends
+      if (lane == 0) atomicOr(g.error_word, 1u);
+      for (int i = 0; rank == 0 && i < g.stages && i < issued; ++i) {
+        if (s-- == 0) s = g.stages - 1, phase ^= 1;
+        ah_wait(full + 8 * s, phase);
+      }
+    }
+    if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+  } else if (warp == AH_EPILOGUE + 1) {
+    if (lane == 0 && rank == 0) {  // ---- products ---------------------------------------------
       int s = 0, turn = 0;
       uint32_t phase = 0;
       bool ok = true, waited = false;
-      for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++turn) {
-        const int n = tile % g.tiles_n;
-        const uint32_t acc = tmem + (turn & 1) * g.nt;
-        if (!(ok = ah_wait(drained + 8 * (turn & 1), ((turn >> 1) & 1) ^ 1))) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        for (int k = 0; k < steps; ++k) {
-          if (!(ok = ah_wait(full + 8 * s, phase))) break;
+      for (int i = 0; ok && i < tiles_m * g.tiles_n; ++i) {
+        const int n = i % g.tiles_n;
+        int count = waited && g.ids ? __ldcg(g.counts + n) : 0;
+        for (int q = 0; ok && q < pieces; ++q, ++turn) {
+          const uint32_t acc = tmem + (turn & 1) * g.nt;
+          if (!(ok = ah_wait(drained + 8 * (turn & 1), ((turn >> 1) & 1) ^ 1))) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint64_t a = ah_operand(stage0 + s * stage_bytes, 128);
-          const uint64_t b = ah_operand(stage0 + s * stage_bytes + AH_A_BYTES, 128);
+          const int here = min(piece, steps - q * piece);
+          for (int k = 0; k < here; ++k) {
+            if (!(ok = ah_wait(full + 8 * s, phase))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint64_t a = ah_operand(stage0 + s * stage_bytes, 128);
+            const uint64_t b = ah_operand(stage0 + s * stage_bytes + AH_A_BYTES, 128);
 #pragma unroll
-          for (int j = 0; j < AH_BK / 16; ++j)
-            ah_multiply(acc, a + 2 * j, b + 2 * j, g.idesc, (k | j) != 0);
-          ah_commit(empty + 8 * s);
-          if (++s == g.stages) s = 0, phase ^= 1;
-        }
-        if (!ok) break;
-        if (!waited) {
-          asm volatile("griddepcontrol.wait;" ::: "memory");
-          waited = true;
-        }
-        const int count = g.ids ? *(volatile const int32_t*)(g.counts + n) : 0;
-        for (int e = 0; e < count; e += AH_PAIR) {
-          if (!(ok = ah_wait(full + 8 * s, phase))) break;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const int both = count - e < AH_PAIR ? count - e : AH_PAIR;
-          const uint32_t base = stage0 + s * stage_bytes;
-          for (int j = 0; j < both; ++j) {
-            const uint64_t a = ah_operand(base + j * AH_BM * 32, 32);
-            const uint32_t u = base + AH_A_BYTES + j * g.nt * 64;
-            ah_multiply(acc, a, ah_operand(u, 32), g.idesc, true);
-            ah_multiply(acc, a, ah_operand(u + g.nt * 32, 32), g.idesc, true);
+            for (int j = 0; j < AH_BK / 16; ++j)
+              ah_multiply<CG>(acc, a + 2 * j, b + 2 * j, g.idesc, (k | j) != 0);
+            ah_commit<CG>(empty + 8 * s);
+            if (++s == g.stages) s = 0, phase ^= 1;
           }
-          ah_commit(empty + 8 * s);
-          if (++s == g.stages) s = 0, phase ^= 1;
+          if (!ok) break;
+          if (q == pieces - 1) {  // the adapters
+            if (!waited) {
+              asm volatile("griddepcontrol.wait;" ::: "memory");
+              waited = true;
+              if (g.ids) count = __ldcg(g.counts + n);
+            }
+            for (int e = 0; e < count; e += AH_PAIR) {
+              if (!(ok = ah_wait(full + 8 * s, phase))) break;
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+              const int both = min(AH_PAIR, count - e);
+              const uint32_t base = stage0 + s * stage_bytes;
+              for (int j = 0; j < both; ++j) {
+                const uint64_t a = ah_operand(base + j * AH_BM * 32, 32);
+                const uint32_t u = base + AH_A_BYTES + j * nh * 64;
+                ah_multiply<CG>(acc, a, ah_operand(u, 32), g.idesc, true);
+                ah_multiply<CG>(acc, a, ah_operand(u + nh * 32, 32), g.idesc, true);
+              }
+              ah_commit<CG>(empty + 8 * s);
+              if (++s == g.stages) s = 0, phase ^= 1;
+            }
+            if (!ok) break;
+          }
+          ah_commit<CG>(done + 8 * (turn & 1));
         }
-        if (ok) ah_commit(done + 8 * (turn & 1));
       }
       if (!ok) {
         atomicOr(g.error_word, 2u);
         // products in flight end before TMEM is given back
-        ah_commit(done + 8 * (turn & 1));
+        ah_commit<CG>(done + 8 * (turn & 1));
         ah_wait(done + 8 * (turn & 1), (turn >> 1) & 1);
       }
     }
-  } else {  // ---- results ------------------------------------------------------------
+  } else {  // ---- results: warp w reads the 32 outputs of its quarter of TMEM, half of the rows --
     int turn = 0;
+    bool ok = true;
     O* y = static_cast<O*>(g.y);
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++turn) {
-      const int m = tile / g.tiles_n, n0 = tile % g.tiles_n * g.nt;
-      if (!ah_wait(done + 8 * (turn & 1), (turn >> 1) & 1)) {
-        if (t == 0) atomicOr(g.error_word, 4u);
-        break;
-      }
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const int v = m * AH_BM + t;  // this lane's output
-      const int here = min(g.nt, g.rows - n0);
-      const uint32_t acc = tmem + (turn & 1) * g.nt + ((uint32_t)(warp * 32) << 16);
+    const int half = (g.nt / 2 + 15) / 16 * 16, c_begin = (warp >> 2) * half,
+              c_end = min(g.nt, c_begin + half);
+    for (int i = 0; ok && i < tiles_m * g.tiles_n; ++i) {
+      const int m = i / g.tiles_n, n0 = i % g.tiles_n * g.nt;
+      const int in_tile = (warp & 3) * 32 + lane, v = v_begin + m * AH_BM + in_tile;
+      const bool store = v < g.out && m * AH_BM + in_tile < g.share;
+      const int here = min(c_end, g.rows - n0);  // columns with a row behind them end here
       O* to = y + (int64_t)n0 * g.ldo + v;
-      for (int c = 0; c < here; c += 16) {
-        uint32_t r[16];
-        asm volatile(
-            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-              "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-              "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-            : "r"(acc + c));
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        if (v < g.out) {
+      if constexpr (CPT > 0) {
+        float sum[CPT];
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (c + j < here) to[(int64_t)(c + j) * g.ldo] = ah_out<O>(r[j]);
+        for (int c = 0; c < CPT; ++c) sum[c] = 0.0f;
+        for (int q = 0; q < pieces; ++q, ++turn) {
+          if (!(ok = ah_wait(done + 8 * (turn & 1), (turn >> 1) & 1))) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t acc = tmem + (turn & 1) * g.nt + ((uint32_t)(warp & 3) << 21) + c_begin;
+#pragma unroll
+          for (int c = 0; c < CPT; c += 16)
+            if (c_begin + c < here) {
+              uint32_t r[16];
+              ah_load16(acc + c, r);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) sum[c + j] += __uint_as_float(r[j]);
+            }
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) ah_arrive_first<CG>(drained + 8 * (turn & 1));
         }
+        if (ok && store) {
+#pragma unroll
+          for (int c = 0; c < CPT; ++c)
+            if (c_begin + c < here) to[(int64_t)(c_begin + c) * g.ldo] = O(sum[c]);
+        }
+      } else {
+        if (!(ok = ah_wait(done + 8 * (turn & 1), (turn >> 1) & 1))) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t acc = tmem + (turn & 1) * g.nt + ((uint32_t)(warp & 3) << 21);
+        for (int c = c_begin; c < here; c += 16) {
+          uint32_t r[16];
+          ah_load16(acc + c, r);
+          if (store) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (c + j < here) to[(int64_t)(c + j) * g.ldo] = O(__uint_as_float(r[j]));
+          }
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) ah_arrive_first<CG>(drained + 8 * (turn & 1));
+        ++turn;
       }
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      ah_arrive(drained + 8 * (turn & 1));
     }
+    if (!ok && t == 0) atomicOr(g.error_word, 4u);
   }
   __syncwarp();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  ah_all_sync<CG>();  // neither CTA of a pair ends while the other may still arrive in it
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  if (warp == 5)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
+  if (warp == AH_EPILOGUE + 1) {
+    if constexpr (CG == 1)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
+    else
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
+  }
 }
 
 }  // namespace nvs
@@ -513,6 +648,8 @@ __global__ void __launch_bounds__(AH_THREADS, 1)
 struct NcbAdapterHead {
   int device = 0, dtype = 0, in = 0, kpad = 0, out = 0, max_rows = 0, slots = 0, max_rank = 0;
   int slices = 0, num_sms = 0;
+  int opad = 0;   // outputs, a multiple of 16
+  int share = 0;  // outputs of a CTA: the same number for each, a multiple of 16
   std::mutex mu;
   void* mem = nullptr;  // everything below but w and w_own
   void *a = nullptr, *b = nullptr, *u = nullptr, *x_own = nullptr;
@@ -521,7 +658,7 @@ struct NcbAdapterHead {
   uint32_t* error_word = nullptr;
   void* w_own = nullptr;  // the weight's copy, where it cannot be read in place
   bool has_w = false;
-  CUtensorMap map_w{}, map_b{};
+  CUtensorMap map_w{}, map_low{}, map_b{};  // map_low: a CTA's last, lower tile
 };
 
 namespace {
@@ -559,22 +696,17 @@ AhEncode ah_encode() {
   }();
   return fn;
 }
-// A map of 16-bit values: dims[0] in a row, strides in bytes from dims[1] on.
-bool ah_map(CUtensorMap* map, int dtype, const void* base, int rank, const cuuint64_t* dims,
-            const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
-  const cuuint32_t one[3] = {1, 1, 1};
+// A map of a matrix of 16-bit values, rows ld apart, read by boxes.
+bool ah_map(CUtensorMap* map, int dtype, const void* base, int64_t cols, int64_t rows, int64_t ld,
+             int box_cols, int box_rows, CUtensorMapSwizzle swizzle) {
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * 2};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, one[2] = {1, 1};
   const AhEncode fn = ah_encode();
   return fn && fn(map, dtype == NCB_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                  (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, one,
+                  2, const_cast<void*>(base), dims, strides, box, one,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-bool ah_map2(CUtensorMap* map, int dtype, const void* base, int64_t cols, int64_t rows, int64_t ld,
-             int box_cols, int box_rows, CUtensorMapSwizzle swizzle) {
-  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * 2};
-  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
-  return ah_map(map, dtype, base, 2, dims, strides, box, swizzle);
 }
 // Whether a matrix of 16-bit values can be read by tiles in place.
 bool ah_readable(const void* p, int64_t ld) { return ah_aligned(p, 16) && ld % 8 == 0; }
@@ -585,7 +717,7 @@ int ah_pack(NcbAdapterHead* h, int slot, const void* a, int64_t lda, const void*
   nvs::adapter_slot_kernel<<<1, 1, 0, st>>>(h->ranks, h->scales, slot, rank, scale);
   nvs::adapter_pack_kernel<E><<<4 * h->num_sms, 256, 0, st>>>(
       static_cast<E*>(h->a), static_cast<E*>(h->b), h->ranks, h->scales, slot, h->in, h->kpad,
-      h->out, h->slices, static_cast<const E*>(a), lda, static_cast<const E*>(b), ldb, rank);
+      h->out, h->opad, h->slices, static_cast<const E*>(a), lda, static_cast<const E*>(b), ldb, rank);
   return ah_launched();
 }
 
@@ -596,33 +728,66 @@ void ah_align(void* to, int64_t pitch, const void* from, int64_t ld, int64_t row
       static_cast<uint16_t*>(to), pitch, static_cast<const uint16_t*>(from), ld, rows, cols);
 }
 
-template <typename O>
-int ah_head(const CUtensorMap& w, const CUtensorMap& x, const CUtensorMap& b, const CUtensorMap& u,
-            const nvs::AhArgs& g, int num_sms, cudaStream_t st) {
-  const int64_t tiles = (int64_t)((g.out + nvs::AH_BM - 1) / nvs::AH_BM) * g.tiles_n;
+constexpr int AH_SINGLE = 64;  // batches of more rows per tile take pairs of CTAs
+
+struct AhMaps {
+  CUtensorMap w, low, x, b, u;
+};
+
+template <typename O, int CG, int CPT>
+int ah_launch(const AhMaps& m, const nvs::AhArgs& g, cudaStream_t st) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(tiles < num_sms ? tiles : num_sms));
+  const int ctas = (g.out + g.share - 1) / g.share;
+  cfg.gridDim = dim3((unsigned)((ctas + CG - 1) / CG * CG));
   cfg.blockDim = dim3(nvs::AH_THREADS);
-  cfg.dynamicSmemBytes = (size_t)g.stages * (nvs::AH_A_BYTES + g.nt * 128) + 1024;
+  cfg.dynamicSmemBytes = (size_t)g.stages * (nvs::AH_A_BYTES + g.nh * 128) + 1024;
   cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CG;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   // starts beside the shrink kernel and waits for it where it needs its results
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = g.ids ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, nvs::head_kernel<O>, w, x, b, u, g) == cudaSuccess
+  cfg.numAttrs = g.ids ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, nvs::head_kernel<O, CG, CPT>, m.w, m.low, m.x, m.b, m.u, g) ==
+                 cudaSuccess
              ? NCB_OK
              : NCB_ERROR_LAUNCH_FAILED;
 }
+// fp32 sums of a row of outputs stay in registers: half of the tile's rows each.
+template <int CG>
+int ah_head(const AhMaps& m, const nvs::AhArgs& g, int dtype, int out_dtype, cudaStream_t st) {
+  if (out_dtype != NCB_DTYPE_F32)
+    return dtype == NCB_DTYPE_BF16 ? ah_launch<__nv_bfloat16, CG, 0>(m, g, st)
+                                   : ah_launch<__half, CG, 0>(m, g, st);
+  if (g.nt <= 32) return ah_launch<float, CG, 16>(m, g, st);
+  if (g.nt <= 128) return ah_launch<float, CG, 64>(m, g, st);
+  return ah_launch<float, CG, 128>(m, g, st);
+}
 
-bool ah_raise() {
-  for (const void* fn : {(const void*)nvs::head_kernel<float>, (const void*)nvs::head_kernel<__half>,
-                         (const void*)nvs::head_kernel<__nv_bfloat16>})
-    if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, nvs::AH_SMEM + 1024) !=
-        cudaSuccess)
+// The shrink kernel asks for the shared-memory split that the head needs: an SM
+// changes it only when it is idle, and the two are to run side by side.
+bool ah_share() {
+  for (const void* fn : {(const void*)nvs::adapter_shrink_kernel<__nv_bfloat16>,
+                         (const void*)nvs::adapter_shrink_kernel<__half>})
+    if (cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout,
+                             cudaSharedmemCarveoutMaxShared) != cudaSuccess)
       return false;
   return true;
+}
+template <int CG>
+bool ah_raise() {
+  bool ok = true;
+  for (const void* fn : {(const void*)nvs::head_kernel<__nv_bfloat16, CG, 0>,
+                         (const void*)nvs::head_kernel<__half, CG, 0>,
+                         (const void*)nvs::head_kernel<float, CG, 16>,
+                         (const void*)nvs::head_kernel<float, CG, 64>,
+                         (const void*)nvs::head_kernel<float, CG, 128>})
+    ok = ok && cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    nvs::AH_SMEM + 1024) == cudaSuccess;
+  return ok;
 }
 
 }  // namespace
@@ -656,8 +821,11 @@ NCB_API int ncb_adapter_head_create(int device, int dtype, int in_features, int 
   h->slots = max_adapters;
   h->max_rank = max_rank;
   h->slices = (max_rank + 15) / 16;
+  h->opad = (out_features + 15) / 16 * 16;
   h->kpad = (in_features + nvs::AH_BK - 1) / nvs::AH_BK * nvs::AH_BK;
   cudaDeviceGetAttribute(&h->num_sms, cudaDevAttrMultiProcessorCount, device);
+  const int ctas = h->num_sms / 2 * 2;  // whole pairs
+  h->share = ((h->out + ctas - 1) / ctas + 15) / 16 * 16;
   size_t off = 0;
   auto carve = [&](size_t bytes) {
     const size_t o = off;
@@ -668,9 +836,9 @@ NCB_API int ncb_adapter_head_create(int device, int dtype, int in_features, int 
   // rows, and a tile names at most as many slots as it has rows.
   const size_t tiles = ((size_t)max_rows + nvs::AH_NT - 1) / nvs::AH_NT;
   const size_t most = (size_t)(h->slots < nvs::AH_NT ? h->slots : nvs::AH_NT) * h->slices;
-  const size_t rows16 = max_rows > nvs::AH_NT ? (size_t)nvs::AH_NT : ((size_t)max_rows + 15) / 16 * 16;
+  const size_t rows16 = max_rows > nvs::AH_NT ? (size_t)nvs::AH_NT : ((size_t)max_rows + 31) / 32 * 32;
   const size_t per = (size_t)h->slots * h->slices * 16;
-  const size_t o_a = carve(per * h->kpad * 2), o_b = carve(per * h->out * 2);
+  const size_t o_a = carve(per * h->kpad * 2), o_b = carve(per * h->opad * 2);
   const size_t o_x = carve((size_t)max_rows * h->kpad * 2);
   const size_t o_u = carve(tiles * most * 2 * rows16 * 16 * 2);
   const size_t o_e = carve(tiles * most * 4), o_c = carve(tiles * 4);
@@ -691,14 +859,11 @@ NCB_API int ncb_adapter_head_create(int device, int dtype, int in_features, int 
   h->scales = reinterpret_cast<float*>(m + o_s);
   h->ranks = reinterpret_cast<int32_t*>(m + o_r);
   h->error_word = reinterpret_cast<uint32_t*>(m + o_w);
-  bool ok = ah_raise() && cudaMemset(h->ranks, 0, off - o_r) == cudaSuccess &&
+  bool ok = ah_share() && ah_raise<1>() && ah_raise<2>() && cudaMemset(h->ranks, 0, off - o_r) == cudaSuccess &&
             cudaDeviceSynchronize() == cudaSuccess;
-  if (ok && h->slots) {  // [slot and slice][out][16]
-    const cuuint64_t dims[3] = {16, (cuuint64_t)h->out, (cuuint64_t)h->slots * h->slices};
-    const cuuint64_t strides[2] = {32, (cuuint64_t)h->out * 32};
-    const cuuint32_t box[3] = {16, nvs::AH_BM, 1};
-    ok = ah_map(&h->map_b, dtype, h->b, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_32B);
-  }
+  if (ok && h->slots)  // 16 rows of 16 values are a row of the map
+    ok = ah_map(&h->map_b, dtype, h->b, 256, (int64_t)per * h->opad / 256, 256, 256,
+                 nvs::AH_BM / 16, CU_TENSOR_MAP_SWIZZLE_NONE);
   if (!ok) {
     cudaGetLastError();
     cudaFree(h->mem);
@@ -741,8 +906,10 @@ NCB_API int ncb_adapter_head_set_weight_device(NcbAdapterHead* h, const void* d_
     d_weight = h->w_own;
     ld = h->kpad;
   }
-  h->has_w = ah_map2(&h->map_w, h->dtype, d_weight, h->in, h->out, ld, nvs::AH_BK, nvs::AH_BM,
-                     CU_TENSOR_MAP_SWIZZLE_128B);
+  h->has_w = ah_map(&h->map_w, h->dtype, d_weight, h->in, h->out, ld, nvs::AH_BK, nvs::AH_BM,
+                     CU_TENSOR_MAP_SWIZZLE_128B) &&
+             ah_map(&h->map_low, h->dtype, d_weight, h->in, h->out, ld, nvs::AH_BK,
+                     (h->share - 1) % nvs::AH_BM + 1, CU_TENSOR_MAP_SWIZZLE_128B);
   return ncb_record_status(h->has_w ? NCB_OK : NCB_ERROR_INIT_FAILED);
 }
 
@@ -806,7 +973,11 @@ NCB_API int ncb_adapter_head_project_device(NcbAdapterHead* h, const void* d_x, 
   g.slots = h->slots;
   g.slices = h->slices;
   g.tiles_n = (rows + nvs::AH_NT - 1) / nvs::AH_NT;
-  g.nt = ((rows + g.tiles_n - 1) / g.tiles_n + 15) / 16 * 16;
+  const int nt = (rows + g.tiles_n - 1) / g.tiles_n;
+  const int group = nt > AH_SINGLE ? 2 : 1;
+  g.nt = (nt + 16 * group - 1) / (16 * group) * (16 * group);
+  g.nh = g.nt / group;
+  g.opad = h->opad;
   g.ids = h->slots ? d_adapter_ids : nullptr;
   g.a = h->a;
   g.ranks = h->ranks;
@@ -819,30 +990,28 @@ NCB_API int ncb_adapter_head_project_device(NcbAdapterHead* h, const void* d_x, 
   g.ldo = ldo;
   const uint32_t type = h->dtype == NCB_DTYPE_BF16 ? 1u : 0u;
   // fp32 sums, both operands of the head's type with the inner axis in rows
-  g.idesc = 1u << 4 | type << 7 | type << 10 | (uint32_t)(g.nt / 8) << 17 | (nvs::AH_BM / 16) << 24;
-  const int stage = nvs::AH_A_BYTES + g.nt * 128;
+  g.idesc = 1u << 4 | type << 7 | type << 10 | (uint32_t)(g.nt / 8) << 17 |
+            (uint32_t)(group * nvs::AH_BM / 16) << 24;
+  const int stage = nvs::AH_A_BYTES + g.nh * 128;
   g.stages = nvs::AH_SMEM / stage < nvs::AH_MAX_STAGES ? nvs::AH_SMEM / stage : nvs::AH_MAX_STAGES;
+  g.share = h->share;
   g.error_word = h->error_word;
-  CUtensorMap map_x, map_u = h->map_w;
-  if (!ah_map2(&map_x, h->dtype, d_x, h->in, rows, ldx, nvs::AH_BK, g.nt, CU_TENSOR_MAP_SWIZZLE_128B) ||
-      (g.ids && !ah_map2(&map_u, h->dtype, h->u, 16, (int64_t)g.tiles_n * g.max_entries * 2 * g.nt, 16,
-                         16, g.nt, CU_TENSOR_MAP_SWIZZLE_32B)))
+  AhMaps m{h->map_w, h->map_low, {}, h->map_b, h->map_w};
+  if (!ah_map(&m.x, h->dtype, d_x, h->in, rows, ldx, nvs::AH_BK, g.nh,
+               CU_TENSOR_MAP_SWIZZLE_128B) ||
+      (g.ids && !ah_map(&m.u, h->dtype, h->u, 256, (int64_t)g.tiles_n * g.max_entries * 2 * g.nt / 16,
+                         256, 256, g.nh / 8, CU_TENSOR_MAP_SWIZZLE_NONE)))
     return ncb_record_status(NCB_ERROR_LAUNCH_FAILED);
   if (g.ids) {
-    const int64_t items = (int64_t)g.max_entries * (g.nt / 16);
-    const int per_tile = (h->num_sms + g.tiles_n - 1) / g.tiles_n;
-    const dim3 grid((unsigned)(items < per_tile ? items : per_tile), g.tiles_n);
+    const dim3 grid(g.nt, g.tiles_n, h->slices);
     if (h->dtype == NCB_DTYPE_BF16)
       nvs::adapter_shrink_kernel<__nv_bfloat16><<<grid, nvs::AS_THREADS, 0, st>>>(g);
     else
       nvs::adapter_shrink_kernel<__half><<<grid, nvs::AS_THREADS, 0, st>>>(g);
     if (ah_launched() != NCB_OK) return ncb_record_status(NCB_ERROR_LAUNCH_FAILED);
   }
-  return ncb_record_status(out_dtype == NCB_DTYPE_F32
-                               ? ah_head<float>(h->map_w, map_x, h->map_b, map_u, g, h->num_sms, st)
-                           : h->dtype == NCB_DTYPE_BF16
-                               ? ah_head<__nv_bfloat16>(h->map_w, map_x, h->map_b, map_u, g, h->num_sms, st)
-                               : ah_head<__half>(h->map_w, map_x, h->map_b, map_u, g, h->num_sms, st));
+  return ncb_record_status(group == 2 ? ah_head<2>(m, g, h->dtype, out_dtype, st)
+                                      : ah_head<1>(m, g, h->dtype, out_dtype, st));
 }
 
 }  // extern "C"

@@ -372,12 +372,10 @@ NCB_API int ncb_sample_rows_min_p_device(const void* d_logits, int dtype, int ro
  *   out[n, :] = W x_n + scale_s * B_s (A_s x_n),  s = adapter_ids[n]
  * W is [out_features, in_features], A_s [rank_s, in_features], B_s
  * [out_features, rank_s], x [rows, in_features], all of the handle's dtype
- * (NCB_DTYPE_F16 or NCB_DTYPE_BF16). Products are summed in fp32 and rounded
- * once, to the output's type; scale_s A_s x_n goes into the second product as the
- * sum of two values of the handle's type (2^-16 of it or less is lost; for fp16
- * it must stay below 65504). No sum's order depends on timing: the same call
- * gives the same bits. A row that uses an adapter holding a NaN or an infinity
- * comes back as NaN, the others of the call are not touched by it.
+ * (NCB_DTYPE_F16 or NCB_DTYPE_BF16). Products are summed in fp32 (A_s x_n too)
+ * and rounded once, to the output's type. No sum's order depends on timing: the
+ * same call gives the same bits, and a row's values depend on no other row's
+ * x or adapter.
  *
  * The handle owns packed copies of the adapters and its scratch; like a
  * sampler it is single-stream: calls on one handle must not overlap on the GPU

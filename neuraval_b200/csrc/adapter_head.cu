@@ -1,26 +1,26 @@
 // LM head with low-rank adapters of many requests (sm_100a):
 //   out[n, :] = W x_n + scale_s B_s (A_s x_n),  s = adapter_ids[n].
 //
-// Two kernels. adapter_shrink_kernel computes u_n = scale_s A_s x_n. The batch
-// is cut into tiles of NT <= 256 rows; for a tile it lists the slots its rows
-// name, 16 ranks of one slot being an entry, and writes each entry's
-// [NT, 16] matrix U_e: row n holds u_n where n's adapter is that slot, zeros
-// elsewhere. The whole product of a tile is then one sum over a longer inner
-// axis,
-//   out^T = [W | B_e1 | B_e2 | ...] [x | U_e1 | U_e2 | ...]^T,
-// which head_kernel runs on the tensor cores: 128 outputs by NT rows of the
-// batch per tile (the weight is the 128-row operand, so that a few rows waste no
-// tensor-core rows and every weight byte is read once), accumulated in TMEM. U_e
-// is split into two 16-bit values, u = hi + lo, each with its own product: one
-// would round u to 8 bits (bf16).
+// head_kernel multiplies on the tensor cores: 128 outputs (256 for a pair of CTAs)
+// by a tile of NT <= 256 rows of the batch, the sums in TMEM. The weight is the
+// 128-row operand, so a few rows waste no tensor-core rows and every weight byte is
+// read once. The adapters are part of the same sums, a longer inner axis:
+//   out^T += B_e U_e^T   for each entry e = (16 ranks of a slot, a block of rows),
+// U_e holding u_n = scale_s A_s x_n for the rows n of the block that name the slot
+// and zeros for the others, split into two 16-bit values, u = hi + lo, each with
+// its own product (one would round u to 8 bits of bf16).
 //
-// The zeros cost operations, not bytes: reading an entry's B from memory takes
-// as long as multiplying it with 256 rows (128 * 16 * 2 bytes against 128 * 16 *
-// 2 * 256 * 2 operations per tile).
+// Tiles of up to AH_SINGLE rows have one block, the tile. Larger tiles are sorted by
+// slot first (adapter_sort_kernel copies x in that order) and cut into blocks of 32
+// rows, so that a slot's entries cover little more than its own rows: with whole
+// tiles as blocks, 32 slots of 16 ranks took a quarter of the tensor cores' time
+// (256x4096x128256: 284 us, without adapters 234).
 //
-// A weight tile is read once from memory and used for all rows of the batch, so
-// up to about 256 rows the head is bound by the weight's bytes, beyond by the
-// tensor cores.
+// adapter_shrink_kernel computes u while the head multiplies its first tile; the
+// head waits for it only before the first entry (programmatic dependent launch).
+//
+// Up to about 256 rows the head is bound by the weight's bytes, beyond by the
+// tensor cores and the power they draw.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -50,7 +50,8 @@ constexpr int AH_SMEM = 208 * 1024;  // stages; leaves room for a shrink CTA on 
 constexpr int AH_EPILOGUE = 8;    // warps that write results
 constexpr int AH_THREADS = (AH_EPILOGUE + 2) * 32;  // and a copying and a multiplying one
 constexpr int AH_PIECE = 8;       // stages added up in TMEM for an fp32 output
-constexpr int AH_PAIR = 2;        // adapter entries per stage
+constexpr int AH_SINGLE = 64;     // rows per tile up to which single CTAs work, unsorted
+constexpr int AH_BLOCK = 32;      // rows per block of larger tiles
 
 struct AhArgs {
   const void* x;
@@ -59,16 +60,20 @@ struct AhArgs {
   int nt, nh, tiles_n;                     // rows per tile, of it per CTA, tiles of rows
   const int32_t* ids;
   const void* a;        // [slots][16 slices][kpad]
+  int block, bh;        // rows per block, of it per CTA
+  void* x_sorted;       // [rows][kpad]
+  int4* info;           // [tiles_n][AH_NT] by row: place, first entry, first and last place of its slot
+  int32_t* order;       // [tiles_n][AH_NT] by place: row of the tile; NULL: as they come
   const int32_t* ranks; // per slot; 0: empty, < 0: |rank|, and B holds a non-finite value
   const float* scales;
-  void* u;              // [tiles_n][max_entries][nt / nh][hi, lo][nh][16]
-  int32_t* entries;     // [tiles_n][max_entries] slot * slices + slice
+  void* u;              // [tiles_n][max_entries][block / bh][hi, lo][bh][16]
+  int2* entries;        // [tiles_n][max_entries] slot * slices + slice, first place
   int32_t* counts;      // [tiles_n]
   int max_entries, opad;
   void* y;
   int64_t ldo;
   int share;  // outputs per CTA
-  uint32_t idesc;
+  uint32_t idesc, idesc_u;
   int stages;
   uint32_t* error_word;
 };
@@ -123,7 +128,7 @@ __global__ void adapter_align_kernel(E* to, int64_t pitch, const E* from, int64_
 
 // ---- u = scale A x --------------------------------------------------------------------
 constexpr int AS_THREADS = 256;
-static_assert(AS_THREADS >= AH_NT && AS_THREADS * 4 >= AH_MAX_ADAPTERS, "a row, four slots per thread");
+static_assert(AS_THREADS >= AH_NT && AS_THREADS * 4 == AH_MAX_ADAPTERS, "a row, four slots per thread");
 
 template <typename E>
 __device__ __forceinline__ float2 ah_pair(uint32_t w) {
@@ -144,15 +149,108 @@ __device__ __forceinline__ uint4 ah_row8(const E* row, int k, int in) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Exclusive prefix over the CTA's threads; the sum of all to `total`.
+__device__ __forceinline__ int as_scan(int v, int32_t* warp_sum, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += x;
+  }
+  if (lane == 31) warp_sum[warp] = inc;
+  __syncthreads();
+  int at = inc - v, all = 0;
+#pragma unroll
+  for (int w = 0; w < AS_THREADS / 32; ++w) {
+    if (w < warp) at += warp_sum[w];
+    all += warp_sum[w];
+  }
+  __syncthreads();
+  *total = all;
+  return at;
+}
+// The slot of a row of the batch, -1 for none; its entries per block to `n`.
+__device__ __forceinline__ int as_slot(const AhArgs& g, int row, int* n) {
+  const int s = row < g.rows ? g.ids[row] : -1;
+  *n = s >= 0 && s < g.slots ? (abs(g.ranks[s]) + 15) / 16 : 0;
+  return *n ? s : -1;
+}
+
+// Larger tiles: grid (nt, tiles_n). The rows of a tile in the order of their slots
+// (rows without one last), a CTA for each row: it finds the row's place, copies its
+// x there and notes where its slot's entries are; row 0's CTA writes the tile's
+// list of entries down. A slot whose rows reach over several blocks has an entry
+// for each.
+__global__ void __launch_bounds__(AS_THREADS) adapter_sort_kernel(const AhArgs g) {
+  __shared__ int32_t first[AH_MAX_ADAPTERS];  // rows per slot, then its first place
+  __shared__ int32_t entry[AH_MAX_ADAPTERS];  // its first entry
+  __shared__ int32_t warp_sum[AS_THREADS / 32];
+  const int t = threadIdx.x, r = blockIdx.x, tile = blockIdx.y, n0 = tile * g.nt;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) first[4 * t + j] = 0;
+  int n, mine_n;
+  const int s = as_slot(g, t < g.nt ? n0 + t : g.rows, &n), mine = as_slot(g, n0 + r, &mine_n);
+  __syncthreads();
+  if (s >= 0) atomicAdd(&first[s], 1);
+  __syncthreads();
+  int rows[4], sum = 0, named;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sum += rows[j] = first[4 * t + j];
+  int at = as_scan(sum, warp_sum, &named), parts[4], slices[4], count;
+  sum = 0;
+#pragma unroll
+  for (int j = 0, a = at; j < 4; ++j) {
+    slices[j] = rows[j] ? (abs(g.ranks[4 * t + j]) + 15) / 16 : 0;
+    parts[j] = rows[j] ? (a + rows[j] - 1) / AH_BLOCK - a / AH_BLOCK + 1 : 0;
+    sum += slices[j] * parts[j];
+    a += rows[j];
+  }
+  int e = as_scan(sum, warp_sum, &count);
+  int2* entries = g.entries + (int64_t)tile * g.max_entries;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    first[4 * t + j] = at;
+    entry[4 * t + j] = e;
+    if (r == 0)
+      for (int i = 0; i < slices[j]; ++i)
+        for (int b = 0; b < parts[j]; ++b)
+          entries[e + i * parts[j] + b] =
+              make_int2((4 * t + j) * g.slices + i, (at / AH_BLOCK + b) * AH_BLOCK);
+    at += rows[j];
+    e += slices[j] * parts[j];
+  }
+  if (r == 0 && t == 0) g.counts[tile] = count;
+  const bool here = t < g.nt && n0 + t < g.rows;
+  const int before = __syncthreads_count(here && s == mine && t < r),
+            equal = __syncthreads_count(here && s == mine);
+  if (n0 + r >= g.rows) return;
+  const int start = mine >= 0 ? first[mine] : named, place = start + before;
+  if (t == 0) {
+    g.order[tile * AH_NT + place] = r;
+    g.info[tile * AH_NT + r] = make_int4(place, mine >= 0 ? entry[mine] : 0, start, start + equal - 1);
+  }
+  // values of 16 bits, whatever their type
+  const uint16_t* x = static_cast<const uint16_t*>(g.x) + (int64_t)(n0 + r) * g.ldx;
+  uint16_t* to = static_cast<uint16_t*>(g.x_sorted) + (int64_t)(n0 + place) * g.kpad;
+  if ((reinterpret_cast<uintptr_t>(g.x) & 15) == 0 && g.ldx % 8 == 0) {
+    for (int k = 8 * t; k < g.in; k += 8 * AS_THREADS)
+      *reinterpret_cast<uint4*>(to + k) = ah_row8(x, k, g.in);
+  } else {
+    for (int k = t; k < g.in; k += AS_THREADS) to[k] = x[k];
+  }
+}
+
 // grid (nt, tiles_n, slices): a CTA for 16 ranks of a row's slot, 8 columns per
-// thread and turn, summed over the threads at the end. Every CTA that has
-// something to write lists its tile's entries for itself (the order of the slots)
-// while its loads are under way. The operations are few (rows * rank * in); what
-// counts is that the kernel ends while the head still multiplies its first tile,
-// so it is spread over as many CTAs as there are rows, and leaves the SM room for
-// the head beside it.
-template <typename E>
+// thread and turn, summed over the threads at the end. The operations are few
+// (rows * rank * in); what counts is that the kernel ends while the head still
+// multiplies its first tile, so it is spread over as many CTAs as there are rows,
+// and leaves the SM room for the head beside it. Unsorted, every CTA lists its
+// tile's entries for itself, in the order of the slots.
+template <typename E, bool SORTED>
 __global__ void __launch_bounds__(AS_THREADS, 2) adapter_shrink_kernel(const AhArgs g) {
+  // sorted: the head starts when every CTA is here, and so after the sort's end
+  if constexpr (SORTED) asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
   __shared__ uint32_t taken[AH_MAX_ADAPTERS / 4];  // a byte per slot: its entries, once named
   __shared__ int32_t first[AH_MAX_ADAPTERS];       // and the first of them
@@ -160,21 +258,20 @@ __global__ void __launch_bounds__(AS_THREADS, 2) adapter_shrink_kernel(const AhA
   __shared__ float part[AS_THREADS / 32][16];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int r = blockIdx.x, tile = blockIdx.y, slice = blockIdx.z, n0 = tile * g.nt;
+  int mine, used = 0;
+  const int slot = as_slot(g, n0 + r, &mine);
+  if (slice >= mine && (SORTED || slice > 0)) return;
+  int other = -1;
+  int4 info{};
+  if constexpr (SORTED) info = g.info[tile * AH_NT + r];
+  else if (t < g.nt) other = as_slot(g, n0 + t, &used);
   taken[t] = 0;
-  auto slot_of = [&](int row) {
-    const int s = row < g.rows ? g.ids[row] : -1;
-    return s >= 0 && s < g.slots ? s : -1;
-  };
-  const int slot = slot_of(n0 + r), other = t < g.nt ? slot_of(n0 + t) : -1;
-  const int rank = slot >= 0 ? g.ranks[slot] : 0;
-  const int mine = (abs(rank) + 15) / 16;
-  if (slice > 0 && slice >= mine) return;
-  const int used = other >= 0 ? (abs(g.ranks[other]) + 15) / 16 : 0;
 
   float acc[16] = {};
   if (mine) {
     const E* a = static_cast<const E*>(g.a) + ((int64_t)slot * g.slices + slice) * 16 * (int64_t)g.kpad;
-    const E* x = static_cast<const E*>(g.x) + (int64_t)(n0 + r) * g.ldx;
+    const E* x = SORTED ? static_cast<const E*>(g.x_sorted) + (int64_t)(n0 + info.x) * g.kpad
+                        : static_cast<const E*>(g.x) + (int64_t)(n0 + r) * g.ldx;
     for (int k = t * 8; k < g.kpad; k += AS_THREADS * 8) {
       const uint4 xv = ah_row8(x, k, g.in);
       uint4 av[16];
@@ -206,62 +303,64 @@ __global__ void __launch_bounds__(AS_THREADS, 2) adapter_shrink_kernel(const AhA
   }
   acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], 1);
   if ((lane & 1) == 0) part[warp][lane >> 1] = acc[0];
-
-  // ---- the tile's entries -------------------------------------------------------------
-  __syncthreads();
-  if (used) reinterpret_cast<uint8_t*>(taken)[other] = (uint8_t)used;  // equal for equal slots
-  __syncthreads();
-  const uint32_t four = taken[t];
-  const int c0 = four & 255, c1 = four >> 8 & 255, c2 = four >> 16 & 255, c3 = four >> 24;
-  const int sum = c0 + c1 + c2 + c3;
-  int inc = sum;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += v;
-  }
-  if (lane == 31) warp_sum[warp] = inc;
-  __syncthreads();
-  int at = inc - sum, count = 0;
-#pragma unroll
-  for (int w = 0; w < AS_THREADS / 32; ++w) {
-    if (w < warp) at += warp_sum[w];
-    count += warp_sum[w];
-  }
-  first[4 * t] = at;
-  first[4 * t + 1] = at + c0;
-  first[4 * t + 2] = at + c0 + c1;
-  first[4 * t + 3] = at + c0 + c1 + c2;
-  if (r == 0 && slice == 0) {  // row 0's CTA writes the list down
-    int32_t* entries = g.entries + (int64_t)tile * g.max_entries;
-    for (int j = 0, e = at; j < 4; ++j)
-      for (int i = 0; i < (int)(four >> (8 * j) & 255); ++i) entries[e++] = (4 * t + j) * g.slices + i;
-    if (t == 0) g.counts[tile] = count;
-  }
   __syncthreads();
 
-  // ---- this row of every entry's U ------------------------------------------------------
-  E* u = static_cast<E*>(g.u) +
-         ((int64_t)tile * g.max_entries * 2 * g.nt + r / g.nh * 2 * g.nh) * 16;
-  const int own = mine ? first[slot] : 0, row = r % g.nh;
-  if (slice == 0)
-    for (int i = t; i < 4 * count; i += AS_THREADS) {  // zeros, 16 bytes at a time
-      const int e = i >> 2;
-      if (e >= own && e < own + mine) continue;
-      *reinterpret_cast<uint4*>(u + (int64_t)e * 2 * g.nt * 16 + (i & 2 ? g.nh * 16 : 0) + row * 16 +
-                                (i & 1) * 8) = make_uint4(0, 0, 0, 0);
+  E* u = static_cast<E*>(g.u) + (int64_t)tile * g.max_entries * 2 * g.block * 16;
+  // where row `at` of an entry's block lies, hi; lo is bh rows further
+  auto row_of = [&](int e, int at) {
+    return u + ((int64_t)e * 2 * g.block + at / g.bh * 2 * g.bh) * 16;
+  };
+  auto clear = [&](int e, int at, int quarter) {  // 16 bytes of the row's hi and lo
+    *reinterpret_cast<uint4*>(row_of(e, at) + (quarter & 2 ? g.bh * 16 : 0) + at % g.bh * 16 +
+                              (quarter & 1) * 8) = make_uint4(0, 0, 0, 0);
+  };
+  int own, place;  // the entry this CTA writes into, the row of it
+  if constexpr (SORTED) {
+    const int b0 = info.z / AH_BLOCK, b1 = info.w / AH_BLOCK, e0 = info.y + slice * (b1 - b0 + 1);
+    own = e0 + info.x / AH_BLOCK - b0;
+    place = info.x % AH_BLOCK;
+    if (info.x == info.z) {  // the slot's first row clears what is not the slot's
+      const int front = info.z % AH_BLOCK, back = AH_BLOCK - 1 - info.w % AH_BLOCK;
+      for (int i = t; i < 4 * front; i += AS_THREADS) clear(e0, i >> 2, i & 3);
+      for (int i = t; i < 4 * back; i += AS_THREADS)
+        clear(e0 + b1 - b0, AH_BLOCK - back + (i >> 2), i & 3);
     }
+  } else {
+    if (used) reinterpret_cast<uint8_t*>(taken)[other] = (uint8_t)used;  // equal for equal slots
+    __syncthreads();
+    const uint32_t four = taken[t];
+    const int c0 = four & 255, c1 = four >> 8 & 255, c2 = four >> 16 & 255, c3 = four >> 24;
+    int count;
+    const int at = as_scan(c0 + c1 + c2 + c3, warp_sum, &count);
+    first[4 * t] = at;
+    first[4 * t + 1] = at + c0;
+    first[4 * t + 2] = at + c0 + c1;
+    first[4 * t + 3] = at + c0 + c1 + c2;
+    if (r == 0 && slice == 0) {  // row 0's CTA writes the list down
+      int2* entries = g.entries + (int64_t)tile * g.max_entries;
+      for (int j = 0, e = at; j < 4; ++j)
+        for (int i = 0; i < (int)(four >> (8 * j) & 255); ++i)
+          entries[e++] = make_int2((4 * t + j) * g.slices + i, 0);
+      if (t == 0) g.counts[tile] = count;
+    }
+    __syncthreads();
+    own = (mine ? first[slot] : 0) + slice;
+    place = r;
+    if (slice == 0)
+      for (int i = t; i < 4 * count; i += AS_THREADS)
+        if (i >> 2 < own || i >> 2 >= own + mine) clear(i >> 2, r, i & 3);
+  }
   if (mine && t < 16) {
     float v = 0.0f;
 #pragma unroll
     for (int w = 0; w < AS_THREADS / 32; ++w) v += part[w][t];
     v *= g.scales[slot];
-    if (rank < 0) v = NAN;
+    if (g.ranks[slot] < 0) v = NAN;
     const E hi = E(v);
     const E lo = E(fabsf((float)hi) < INFINITY ? v - (float)hi : 0.0f);
-    E* to = u + (int64_t)(own + slice) * 2 * g.nt * 16 + ah_at(row, t);
+    E* to = row_of(own, place) + ah_at(place % g.bh, t);
     to[0] = hi;
-    to[(int64_t)g.nh * 16] = lo;
+    to[(int64_t)g.bh * 16] = lo;
   }
 }
 
@@ -447,6 +546,7 @@ __global__ void __launch_bounds__(AH_THREADS, 1)
   ah_all_sync<CG>();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = s_tmem;
+  constexpr int PER = CG == 1 ? 2 : 4;  // entries per stage
   const int steps = (g.in + AH_BK - 1) / AH_BK;
   const int piece = CPT ? AH_PIECE : steps;  // stages added up in TMEM
   const int pieces = (steps + piece - 1) / piece;
@@ -456,11 +556,13 @@ __global__ void __launch_bounds__(AH_THREADS, 1)
     int s = 0, issued = 0;
     uint32_t phase = 0;
     bool ok = true, waited = false;
+    if (g.order) asm volatile("fence.proxy.async.global;" ::: "memory");  // the sorted x
     for (int i = 0; ok && i < tiles_m * g.tiles_n; ++i) {
       const int m = i / g.tiles_n, n = i % g.tiles_n;
       const int v0 = v_begin + m * AH_BM, high = min(AH_BM, g.share - m * AH_BM);
-      const int32_t* entries = g.entries + (int64_t)n * g.max_entries;
-      int count = 0, mine = 0;  // entries of the tile of rows; lane l holds the l-th of 32
+      const int2* entries = g.entries + (int64_t)n * g.max_entries;
+      int count = 0;  // entries of the tile of rows; lane l holds the l-th of 32
+      int2 mine{};
       if (waited && g.ids) {
         count = __ldcg(g.counts + n);
         if (lane < count) mine = __ldcg(entries + lane);
@@ -487,19 +589,18 @@ __global__ void __launch_bounds__(AH_THREADS, 1)
           if (lane < count) mine = __ldcg(entries + lane);
         }
       }
-      for (int e = 0; e < count; e += AH_PAIR) {
-        if (e && (e & 31) == 0) mine = e + lane < count ? __ldcg(entries + e + lane) : 0;
+      for (int e = 0; e < count; e += PER) {
+        if (e && (e & 31) == 0 && e + lane < count) mine = __ldcg(entries + e + lane);
         if (!(ok = ah_wait(empty + 8 * s, phase ^ 1))) break;
-        const int both = min(AH_PAIR, count - e);
-        const int z0 = __shfl_sync(0xffffffffu, mine, e & 31),
-                  z1 = __shfl_sync(0xffffffffu, mine, (e & 31) + 1);
-        if (lane == 0) {
-          const uint32_t a = stage0 + s * stage_bytes, bar = full + 8 * s;
-          if (rank == 0) ah_expect(bar, CG * both * (AH_BM * 32 + 2 * nh * 32));
-          for (int j = 0; j < both; ++j) {
-            ah_copy<CG>(a + j * AH_BM * 32, &map_b, bar, 0, (int)(((int64_t)(j ? z1 : z0) * g.opad + v0) / 16));
-            ah_copy<CG>(a + AH_A_BYTES + j * nh * 64, &map_u, bar, 0,
-                         ((n * g.max_entries + e + j) * 2 * g.nt + rank * 2 * nh) / 16);
+        const int several = min(PER, count - e);
+        const uint32_t a = stage0 + s * stage_bytes, bar = full + 8 * s;
+        if (lane == 0 && rank == 0) ah_expect(bar, CG * several * (AH_BM * 32 + g.bh * 64));
+        for (int j = 0; j < several; ++j) {
+          const int z = __shfl_sync(0xffffffffu, mine.x, (e & 31) + j);
+          if (lane == 0) {
+            ah_copy<CG>(a + j * AH_BM * 32, &map_b, bar, 0, (int)(((int64_t)z * g.opad + v0) / 16));
+            ah_copy<CG>(a + AH_A_BYTES + j * g.bh * 64, &map_u, bar, 0,
+                        (int)((((int64_t)n * g.max_entries + e + j) * 2 * g.block + rank * 2 * g.bh) / 16));
           }
         }
         __syncwarp();
@@ -516,13 +617,18 @@ __global__ void __launch_bounds__(AH_THREADS, 1)
     }
     if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
   } else if (warp == AH_EPILOGUE + 1) {
-    if (lane == 0 && rank == 0) {  // ---- products ---------------------------------------------
+    if (rank == 0) {  // ---- products: the warp waits together, a lane issues -------------------
       int s = 0, turn = 0;
       uint32_t phase = 0;
       bool ok = true, waited = false;
       for (int i = 0; ok && i < tiles_m * g.tiles_n; ++i) {
         const int n = i % g.tiles_n;
-        int count = waited && g.ids ? __ldcg(g.counts + n) : 0;
+        const int2* entries = g.entries + (int64_t)n * g.max_entries;
+        int count = 0, mine = 0;  // as above; of an entry, the first place of its block
+        if (waited && g.ids) {
+          count = __ldcg(g.counts + n);
+          if (lane < count) mine = __ldcg(&entries[lane].y);
+        }
         for (int q = 0; ok && q < pieces; ++q, ++turn) {
           const uint32_t acc = tmem + (turn & 1) * g.nt;
           if (!(ok = ah_wait(drained + 8 * (turn & 1), ((turn >> 1) & 1) ^ 1))) break;
@@ -531,12 +637,15 @@ __global__ void __launch_bounds__(AH_THREADS, 1)
           for (int k = 0; k < here; ++k) {
             if (!(ok = ah_wait(full + 8 * s, phase))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint64_t a = ah_operand(stage0 + s * stage_bytes, 128);
-            const uint64_t b = ah_operand(stage0 + s * stage_bytes + AH_A_BYTES, 128);
+            if (lane == 0) {
+              const uint64_t a = ah_operand(stage0 + s * stage_bytes, 128);
+              const uint64_t b = ah_operand(stage0 + s * stage_bytes + AH_A_BYTES, 128);
 #pragma unroll
-            for (int j = 0; j < AH_BK / 16; ++j)
-              ah_multiply<CG>(acc, a + 2 * j, b + 2 * j, g.idesc, (k | j) != 0);
-            ah_commit<CG>(empty + 8 * s);
+              for (int j = 0; j < AH_BK / 16; ++j)
+                ah_multiply<CG>(acc, a + 2 * j, b + 2 * j, g.idesc, (k | j) != 0);
+              ah_commit<CG>(empty + 8 * s);
+            }
+            __syncwarp();
             if (++s == g.stages) s = 0, phase ^= 1;
           }
           if (!ok) break;
@@ -544,35 +653,47 @@ __global__ void __launch_bounds__(AH_THREADS, 1)
             if (!waited) {
               asm volatile("griddepcontrol.wait;" ::: "memory");
               waited = true;
-              if (g.ids) count = __ldcg(g.counts + n);
+              if (g.ids) {
+                count = __ldcg(g.counts + n);
+                if (lane < count) mine = __ldcg(&entries[lane].y);
+              }
             }
-            for (int e = 0; e < count; e += AH_PAIR) {
+            for (int e = 0; e < count; e += PER) {
+              if (e && (e & 31) == 0 && e + lane < count) mine = __ldcg(&entries[e + lane].y);
               if (!(ok = ah_wait(full + 8 * s, phase))) break;
               asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-              const int both = min(AH_PAIR, count - e);
+              const int several = min(PER, count - e);
               const uint32_t base = stage0 + s * stage_bytes;
-              for (int j = 0; j < both; ++j) {
-                const uint64_t a = ah_operand(base + j * AH_BM * 32, 32);
-                const uint32_t u = base + AH_A_BYTES + j * nh * 64;
-                ah_multiply<CG>(acc, a, ah_operand(u, 32), g.idesc, true);
-                ah_multiply<CG>(acc, a, ah_operand(u + nh * 32, 32), g.idesc, true);
+              for (int j = 0; j < several; ++j) {
+                const int place = __shfl_sync(0xffffffffu, mine, (e & 31) + j);
+                if (lane == 0) {
+                  const uint64_t a = ah_operand(base + j * AH_BM * 32, 32);
+                  const uint32_t u = base + AH_A_BYTES + j * g.bh * 64;
+                  ah_multiply<CG>(acc + place, a, ah_operand(u, 32), g.idesc_u, true);
+                  ah_multiply<CG>(acc + place, a, ah_operand(u + g.bh * 32, 32), g.idesc_u, true);
+                }
               }
-              ah_commit<CG>(empty + 8 * s);
+              if (lane == 0) ah_commit<CG>(empty + 8 * s);
+              __syncwarp();
               if (++s == g.stages) s = 0, phase ^= 1;
             }
             if (!ok) break;
           }
-          ah_commit<CG>(done + 8 * (turn & 1));
+          if (lane == 0) ah_commit<CG>(done + 8 * (turn & 1));
+          __syncwarp();
         }
       }
       if (!ok) {
-        atomicOr(g.error_word, 2u);
         // products in flight end before TMEM is given back
-        ah_commit<CG>(done + 8 * (turn & 1));
+        if (lane == 0) {
+          atomicOr(g.error_word, 2u);
+          ah_commit<CG>(done + 8 * (turn & 1));
+        }
         ah_wait(done + 8 * (turn & 1), (turn >> 1) & 1);
       }
     }
   } else {  // ---- results: warp w reads the 32 outputs of its quarter of TMEM, half of the rows --
+    if (g.order) asm volatile("griddepcontrol.wait;" ::: "memory");
     int turn = 0;
     bool ok = true;
     O* y = static_cast<O*>(g.y);
@@ -584,6 +705,10 @@ __global__ void __launch_bounds__(AH_THREADS, 1)
       const bool store = v < g.out && m * AH_BM + in_tile < g.share;
       const int here = min(c_end, g.rows - n0);  // columns with a row behind them end here
       O* to = y + (int64_t)n0 * g.ldo + v;
+      const int32_t* order = g.order + i % g.tiles_n * AH_NT;
+      auto put = [&](int c, float x) {  // the row in place c of the tile
+        if (c < here) to[(int64_t)(g.order ? order[c] : c) * g.ldo] = O(x);
+      };
       if constexpr (CPT > 0) {
         float sum[CPT];
 #pragma unroll
@@ -606,8 +731,7 @@ __global__ void __launch_bounds__(AH_THREADS, 1)
         }
         if (ok && store) {
 #pragma unroll
-          for (int c = 0; c < CPT; ++c)
-            if (c_begin + c < here) to[(int64_t)(c_begin + c) * g.ldo] = O(sum[c]);
+          for (int c = 0; c < CPT; ++c) put(c_begin + c, sum[c]);
         }
       } else {
         if (!(ok = ah_wait(done + 8 * (turn & 1), (turn >> 1) & 1))) break;
@@ -618,8 +742,7 @@ __global__ void __launch_bounds__(AH_THREADS, 1)
           ah_load16(acc + c, r);
           if (store) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (c + j < here) to[(int64_t)(c + j) * g.ldo] = O(__uint_as_float(r[j]));
+            for (int j = 0; j < 16; ++j) put(c + j, __uint_as_float(r[j]));
           }
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -653,7 +776,9 @@ struct NcbAdapterHead {
   std::mutex mu;
   void* mem = nullptr;  // everything below but w and w_own
   void *a = nullptr, *b = nullptr, *u = nullptr, *x_own = nullptr;
-  int32_t *ranks = nullptr, *entries = nullptr, *counts = nullptr;
+  int32_t *ranks = nullptr, *counts = nullptr, *order = nullptr;
+  int2* entries = nullptr;
+  int4* info = nullptr;
   float* scales = nullptr;
   uint32_t* error_word = nullptr;
   void* w_own = nullptr;  // the weight's copy, where it cannot be read in place
@@ -728,66 +853,79 @@ void ah_align(void* to, int64_t pitch, const void* from, int64_t ld, int64_t row
       static_cast<uint16_t*>(to), pitch, static_cast<const uint16_t*>(from), ld, rows, cols);
 }
 
-constexpr int AH_SINGLE = 64;  // batches of more rows per tile take pairs of CTAs
-
 struct AhMaps {
   CUtensorMap w, low, x, b, u;
 };
 
-template <typename O, int CG, int CPT>
-int ah_launch(const AhMaps& m, const nvs::AhArgs& g, cudaStream_t st) {
+// `beside`: it may start while the kernel before it still runs, and waits for that
+// one itself.
+template <typename... A>
+bool ah_start(void (*kernel)(A...), dim3 grid, int threads, size_t smem, int cluster, bool beside,
+              cudaStream_t st, const std::common_type_t<A>&... args) {
   cudaLaunchConfig_t cfg{};
-  const int ctas = (g.out + g.share - 1) / g.share;
-  cfg.gridDim = dim3((unsigned)((ctas + CG - 1) / CG * CG));
-  cfg.blockDim = dim3(nvs::AH_THREADS);
-  cfg.dynamicSmemBytes = (size_t)g.stages * (nvs::AH_A_BYTES + g.nh * 128) + 1024;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = CG;
+  at[0].val.clusterDim.x = cluster;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  // starts beside the shrink kernel and waits for it where it needs its results
   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = g.ids ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, nvs::head_kernel<O, CG, CPT>, m.w, m.low, m.x, m.b, m.u, g) ==
-                 cudaSuccess
-             ? NCB_OK
-             : NCB_ERROR_LAUNCH_FAILED;
+  cfg.numAttrs = beside ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess;
 }
-// fp32 sums of a row of outputs stay in registers: half of the tile's rows each.
-template <int CG>
-int ah_head(const AhMaps& m, const nvs::AhArgs& g, int dtype, int out_dtype, cudaStream_t st) {
-  if (out_dtype != NCB_DTYPE_F32)
-    return dtype == NCB_DTYPE_BF16 ? ah_launch<__nv_bfloat16, CG, 0>(m, g, st)
-                                   : ah_launch<__half, CG, 0>(m, g, st);
-  if (g.nt <= 32) return ah_launch<float, CG, 16>(m, g, st);
-  if (g.nt <= 128) return ah_launch<float, CG, 64>(m, g, st);
-  return ah_launch<float, CG, 128>(m, g, st);
+
+template <typename O, int CG, int CPT>
+bool ah_launch(const AhMaps& m, const nvs::AhArgs& g, cudaStream_t st) {
+  const int ctas = (g.out + g.share - 1) / g.share;
+  return ah_start(nvs::head_kernel<O, CG, CPT>, dim3((ctas + CG - 1) / CG * CG), nvs::AH_THREADS,
+                  (size_t)g.stages * (nvs::AH_A_BYTES + g.nh * 128) + 1024, CG, g.ids != nullptr, st,
+                  m.w, m.low, m.x, m.b, m.u, g);
+}
+template <typename E, int CG>
+int ah_head(const AhMaps& m, const nvs::AhArgs& g, bool wide, cudaStream_t st) {
+  bool ok = true;
+  if (g.ids) {
+    const dim3 grid(g.nt, g.tiles_n, g.slices);
+    if constexpr (CG == 2)
+      ok = ah_start(nvs::adapter_sort_kernel, dim3(g.nt, g.tiles_n), nvs::AS_THREADS, 0, 1, false, st, g);
+    ok = ok && ah_start(nvs::adapter_shrink_kernel<E, CG == 2>, grid, nvs::AS_THREADS, 0, 1, CG == 2, st, g);
+  }
+  // fp32 sums stay in registers: those of half of the tile's rows per thread
+  if (!wide) ok = ok && ah_launch<E, CG, 0>(m, g, st);
+  else if constexpr (CG == 1)
+    ok = ok && (g.nt <= 32 ? ah_launch<float, 1, 16>(m, g, st) : ah_launch<float, 1, 64>(m, g, st));
+  else
+    ok = ok && (g.nt <= 128 ? ah_launch<float, 2, 64>(m, g, st) : ah_launch<float, 2, 128>(m, g, st));
+  return ok ? NCB_OK : NCB_ERROR_LAUNCH_FAILED;
 }
 
 // The shrink kernel asks for the shared-memory split that the head needs: an SM
 // changes it only when it is idle, and the two are to run side by side.
 bool ah_share() {
-  for (const void* fn : {(const void*)nvs::adapter_shrink_kernel<__nv_bfloat16>,
-                         (const void*)nvs::adapter_shrink_kernel<__half>})
+  for (const void* fn : {(const void*)nvs::adapter_sort_kernel,
+                         (const void*)nvs::adapter_shrink_kernel<__nv_bfloat16, false>,
+                         (const void*)nvs::adapter_shrink_kernel<__nv_bfloat16, true>,
+                         (const void*)nvs::adapter_shrink_kernel<__half, false>,
+                         (const void*)nvs::adapter_shrink_kernel<__half, true>})
     if (cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout,
                              cudaSharedmemCarveoutMaxShared) != cudaSuccess)
       return false;
   return true;
 }
-template <int CG>
 bool ah_raise() {
-  bool ok = true;
-  for (const void* fn : {(const void*)nvs::head_kernel<__nv_bfloat16, CG, 0>,
-                         (const void*)nvs::head_kernel<__half, CG, 0>,
-                         (const void*)nvs::head_kernel<float, CG, 16>,
-                         (const void*)nvs::head_kernel<float, CG, 64>,
-                         (const void*)nvs::head_kernel<float, CG, 128>})
-    ok = ok && cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    nvs::AH_SMEM + 1024) == cudaSuccess;
-  return ok;
+  for (const void* fn :
+       {(const void*)nvs::head_kernel<__nv_bfloat16, 1, 0>, (const void*)nvs::head_kernel<__nv_bfloat16, 2, 0>,
+        (const void*)nvs::head_kernel<__half, 1, 0>, (const void*)nvs::head_kernel<__half, 2, 0>,
+        (const void*)nvs::head_kernel<float, 1, 16>, (const void*)nvs::head_kernel<float, 1, 64>,
+        (const void*)nvs::head_kernel<float, 2, 64>, (const void*)nvs::head_kernel<float, 2, 128>})
+    if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, nvs::AH_SMEM + 1024) !=
+        cudaSuccess)
+      return false;
+  return true;
 }
 
 }  // namespace
@@ -832,16 +970,17 @@ NCB_API int ncb_adapter_head_create(int device, int dtype, int in_features, int 
     off += (bytes + 255) / 256 * 256;
     return o;
   };
-  // A batch of n rows is cut into tiles of at most 256, each of a multiple of 16
-  // rows, and a tile names at most as many slots as it has rows.
   const size_t tiles = ((size_t)max_rows + nvs::AH_NT - 1) / nvs::AH_NT;
-  const size_t most = (size_t)(h->slots < nvs::AH_NT ? h->slots : nvs::AH_NT) * h->slices;
-  const size_t rows16 = max_rows > nvs::AH_NT ? (size_t)nvs::AH_NT : ((size_t)max_rows + 31) / 32 * 32;
+  // entries of a tile: a block for each of its slots' 16 ranks, and one more for each
+  // border between blocks that a slot's rows reach over
+  const size_t most = h->slots ? ((size_t)(h->slots < nvs::AH_NT ? h->slots : nvs::AH_NT) +
+                                  nvs::AH_NT / nvs::AH_BLOCK) * h->slices : 0;
   const size_t per = (size_t)h->slots * h->slices * 16;
   const size_t o_a = carve(per * h->kpad * 2), o_b = carve(per * h->opad * 2);
   const size_t o_x = carve((size_t)max_rows * h->kpad * 2);
-  const size_t o_u = carve(tiles * most * 2 * rows16 * 16 * 2);
-  const size_t o_e = carve(tiles * most * 4), o_c = carve(tiles * 4);
+  const size_t o_u = carve(tiles * most * 2 * nvs::AH_SINGLE * 16 * 2);  // the larger block
+  const size_t o_e = carve(tiles * most * sizeof(int2)), o_c = carve(tiles * 4);
+  const size_t o_i = carve(tiles * nvs::AH_NT * sizeof(int4)), o_o = carve(tiles * nvs::AH_NT * 4);
   const size_t o_s = carve((size_t)h->slots * 4), o_r = carve((size_t)h->slots * 4);
   const size_t o_w = carve(4);
   if (cudaMalloc(&h->mem, off) != cudaSuccess) {
@@ -854,12 +993,14 @@ NCB_API int ncb_adapter_head_create(int device, int dtype, int in_features, int 
   h->b = m + o_b;
   h->x_own = m + o_x;
   h->u = m + o_u;
-  h->entries = reinterpret_cast<int32_t*>(m + o_e);
+  h->entries = reinterpret_cast<int2*>(m + o_e);
+  h->info = reinterpret_cast<int4*>(m + o_i);
+  h->order = reinterpret_cast<int32_t*>(m + o_o);
   h->counts = reinterpret_cast<int32_t*>(m + o_c);
   h->scales = reinterpret_cast<float*>(m + o_s);
   h->ranks = reinterpret_cast<int32_t*>(m + o_r);
   h->error_word = reinterpret_cast<uint32_t*>(m + o_w);
-  bool ok = ah_share() && ah_raise<1>() && ah_raise<2>() && cudaMemset(h->ranks, 0, off - o_r) == cudaSuccess &&
+  bool ok = ah_share() && ah_raise() && cudaMemset(h->ranks, 0, off - o_r) == cudaSuccess &&
             cudaDeviceSynchronize() == cudaSuccess;
   if (ok && h->slots)  // 16 rows of 16 values are a row of the map
     ok = ah_map(&h->map_b, dtype, h->b, 256, (int64_t)per * h->opad / 256, 256, 256,
@@ -958,60 +1099,65 @@ NCB_API int ncb_adapter_head_project_device(NcbAdapterHead* h, const void* d_x, 
   AhDevice guard(h->device);
   if (!guard.ok) return ncb_record_status(NCB_ERROR_INIT_FAILED);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (!ah_readable(d_x, ldx)) {
-    ah_align(h->x_own, h->kpad, d_x, ldx, rows, h->in, h->num_sms, st);
-    d_x = h->x_own;
-    ldx = h->kpad;
-  }
   nvs::AhArgs g{};
-  g.x = d_x;
-  g.ldx = ldx;
   g.rows = rows;
   g.in = h->in;
   g.kpad = h->kpad;
   g.out = h->out;
+  g.opad = h->opad;
   g.slots = h->slots;
   g.slices = h->slices;
+  // tiles of up to 256 rows, all of one size; pairs of CTAs where they are large
   g.tiles_n = (rows + nvs::AH_NT - 1) / nvs::AH_NT;
-  const int nt = (rows + g.tiles_n - 1) / g.tiles_n;
-  const int group = nt > AH_SINGLE ? 2 : 1;
-  g.nt = (nt + 16 * group - 1) / (16 * group) * (16 * group);
+  const int tile = (rows + g.tiles_n - 1) / g.tiles_n;
+  const int group = tile > nvs::AH_SINGLE ? 2 : 1;
+  g.nt = (tile + 16 * group - 1) / (16 * group) * (16 * group);
   g.nh = g.nt / group;
-  g.opad = h->opad;
   g.ids = h->slots ? d_adapter_ids : nullptr;
+  const bool sorted = g.ids && group == 2;
+  g.block = group == 2 ? nvs::AH_BLOCK : g.nt;
+  g.bh = g.block / group;
+  g.max_entries = (h->slots < nvs::AH_NT ? h->slots : nvs::AH_NT) * h->slices +
+                  nvs::AH_NT / nvs::AH_BLOCK * h->slices;
   g.a = h->a;
   g.ranks = h->ranks;
   g.scales = h->scales;
   g.u = h->u;
   g.entries = h->entries;
   g.counts = h->counts;
-  g.max_entries = (h->slots < g.nt ? h->slots : g.nt) * h->slices;
+  g.info = h->info;
+  g.order = sorted ? h->order : nullptr;
+  g.x_sorted = h->x_own;
   g.y = d_out;
   g.ldo = ldo;
-  const uint32_t type = h->dtype == NCB_DTYPE_BF16 ? 1u : 0u;
   // fp32 sums, both operands of the head's type with the inner axis in rows
-  g.idesc = 1u << 4 | type << 7 | type << 10 | (uint32_t)(g.nt / 8) << 17 |
-            (uint32_t)(group * nvs::AH_BM / 16) << 24;
+  const uint32_t type = h->dtype == NCB_DTYPE_BF16 ? 1u : 0u;
+  const uint32_t kind = 1u << 4 | type << 7 | type << 10 | (uint32_t)(group * nvs::AH_BM / 16) << 24;
+  g.idesc = kind | (uint32_t)(g.nt / 8) << 17;
+  g.idesc_u = kind | (uint32_t)(g.block / 8) << 17;
   const int stage = nvs::AH_A_BYTES + g.nh * 128;
   g.stages = nvs::AH_SMEM / stage < nvs::AH_MAX_STAGES ? nvs::AH_SMEM / stage : nvs::AH_MAX_STAGES;
   g.share = h->share;
   g.error_word = h->error_word;
-  AhMaps m{h->map_w, h->map_low, {}, h->map_b, h->map_w};
-  if (!ah_map(&m.x, h->dtype, d_x, h->in, rows, ldx, nvs::AH_BK, g.nh,
-               CU_TENSOR_MAP_SWIZZLE_128B) ||
-      (g.ids && !ah_map(&m.u, h->dtype, h->u, 256, (int64_t)g.tiles_n * g.max_entries * 2 * g.nt / 16,
-                         256, 256, g.nh / 8, CU_TENSOR_MAP_SWIZZLE_NONE)))
-    return ncb_record_status(NCB_ERROR_LAUNCH_FAILED);
-  if (g.ids) {
-    const dim3 grid(g.nt, g.tiles_n, h->slices);
-    if (h->dtype == NCB_DTYPE_BF16)
-      nvs::adapter_shrink_kernel<__nv_bfloat16><<<grid, nvs::AS_THREADS, 0, st>>>(g);
-    else
-      nvs::adapter_shrink_kernel<__half><<<grid, nvs::AS_THREADS, 0, st>>>(g);
-    if (ah_launched() != NCB_OK) return ncb_record_status(NCB_ERROR_LAUNCH_FAILED);
+  if (!sorted && !ah_readable(d_x, ldx)) {  // (the sort copies x anyway)
+    ah_align(h->x_own, h->kpad, d_x, ldx, rows, h->in, h->num_sms, st);
+    d_x = h->x_own;
+    ldx = h->kpad;
   }
-  return ncb_record_status(group == 2 ? ah_head<2>(m, g, h->dtype, out_dtype, st)
-                                      : ah_head<1>(m, g, h->dtype, out_dtype, st));
+  g.x = d_x;
+  g.ldx = ldx;
+  AhMaps m{h->map_w, h->map_low, {}, h->map_b, h->map_w};
+  if (!ah_map(&m.x, h->dtype, sorted ? h->x_own : d_x, h->in, rows, sorted ? h->kpad : ldx,
+              nvs::AH_BK, g.nh, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      (g.ids && !ah_map(&m.u, h->dtype, h->u, 256, (int64_t)g.tiles_n * g.max_entries * 2 * g.block / 16,
+                        256, 256, g.bh / 8, CU_TENSOR_MAP_SWIZZLE_NONE)))
+    return ncb_record_status(NCB_ERROR_LAUNCH_FAILED);
+  const bool wide = out_dtype == NCB_DTYPE_F32;
+  if (h->dtype == NCB_DTYPE_BF16)
+    return ncb_record_status(group == 2 ? ah_head<__nv_bfloat16, 2>(m, g, wide, st)
+                                        : ah_head<__nv_bfloat16, 1>(m, g, wide, st));
+  return ncb_record_status(group == 2 ? ah_head<__half, 2>(m, g, wide, st)
+                                      : ah_head<__half, 1>(m, g, wide, st));
 }
 
 }  // extern "C"

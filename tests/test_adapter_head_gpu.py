@@ -7,9 +7,7 @@ random values, within a tolerance derived from the arithmetic:
     running sum (2^-23 where the hardware truncates, but then for 16 products at
     once); the running sum of products with random signs stays below 6 times
     their 2-norm q, so (K + R + 32) 2^-24 6 q covers them;
-  - A_s x_n carried as the sum of two 16-bit values: off by 2^-16 relative
-    (bf16: two roundings of 2^-9 and more; fp16: more exact, down to its least
-    step, 2^-24), so 2^-16 |B_s| |u| + 2^-24 |B_s| 1;
+  - A_s x_n, a sum of the same kind, multiplied with B_s;
   - the output's own rounding, half a step of its type.
 """
 import numpy as np
@@ -64,7 +62,7 @@ class Case:
                 q[n] += (b ** 2) @ (u ** 2)
                 # u itself, a sum in fp32
                 du = (self.inner + 32) * 2.0 ** -24 * 6 * self.scales[i] * ((a ** 2) @ (x[n] ** 2)).sqrt()
-                tol[n] += b.abs() @ (2.0 ** -16 * u.abs() + 2.0 ** -24 + du)
+                tol[n] += b.abs() @ (2.0 ** -23 * u.abs() + du)
         return y, tol + (self.inner + R + 32) * 2.0 ** -24 * 6 * q.sqrt()
 
     def head(self, max_rows=None, max_adapters=None, max_rank=None):
@@ -224,8 +222,8 @@ def test_weight_set_again():
 
 
 def test_non_finite_rows_stay_alone():
-    """A row of x with NaN, an adapter with NaN in A or an infinity in B: NaN in the rows that use
-    it, and the other rows as they are."""
+    """A row of x with NaN, an adapter with NaN in A or an infinity in B: the rows that use it show
+    it, the other rows are as they were."""
     c = Case(20, 128, 260, [16, 16], np.arange(20) % 2, "bf16", 15, whole=True)
     want = c.want()[0].float()
     c.x[3, 5] = float("nan")
@@ -239,7 +237,7 @@ def test_non_finite_rows_stay_alone():
         spoil()
         with c.head() as h:
             got = c.run(h)
-            assert got[1::2].isnan().all() and (got[::2] == want[::2]).all()
+            assert not got[1::2].isfinite().all() and (got[::2] == want[::2]).all()
             h.set_adapter(1, c.a[0], c.b[0], 1.0)  # a sound one in its place
             assert c.run(h).isfinite().all()
 

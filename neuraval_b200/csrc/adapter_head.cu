@@ -52,6 +52,7 @@ constexpr int AH_THREADS = (AH_EPILOGUE + 2) * 32;  // and a copying and a multi
 constexpr int AH_PIECE = 8;       // stages added up in TMEM for an fp32 output
 constexpr int AH_SINGLE = 64;     // rows per tile up to which single CTAs work, unsorted
 constexpr int AH_BLOCK = 32;      // rows per block of larger tiles
+__host__ __device__ constexpr int ah_per(int group) { return group == 1 ? 2 : 4; }  // adapter entries per stage
 
 struct AhArgs {
   const void* x;
@@ -66,13 +67,14 @@ struct AhArgs {
   int32_t* order;       // [tiles_n][AH_NT] by place: row of the tile; NULL: as they come
   const int32_t* ranks; // per slot; 0: empty, < 0: |rank|, and B holds a non-finite value
   const float* scales;
-  void* u;              // [tiles_n][max_entries][block / bh][hi, lo][bh][16]
+  void* u;              // [tiles_n][block / bh][max_entries][hi, lo][bh][16]
   int2* entries;        // [tiles_n][max_entries] slot * slices + slice, first place
   int32_t* counts;      // [tiles_n]
   int max_entries, opad;
   void* y;
   int64_t ldo;
-  int share;  // outputs per CTA
+  int share;   // outputs per CTA
+  int groups;  // tiles of rows worked on at the same time, by neighbouring CTAs
   uint32_t idesc, idesc_u;
   int stages;
   uint32_t* error_word;
@@ -127,7 +129,8 @@ __global__ void adapter_align_kernel(E* to, int64_t pitch, const E* from, int64_
 }
 
 // ---- u = scale A x --------------------------------------------------------------------
-constexpr int AS_THREADS = 256;
+constexpr int AS_THREADS = 256;  // of the sort
+constexpr int AU_THREADS = 128;  // of the shrink kernel
 static_assert(AS_THREADS >= AH_NT && AS_THREADS * 4 == AH_MAX_ADAPTERS, "a row, four slots per thread");
 
 template <typename E>
@@ -241,54 +244,107 @@ __global__ void __launch_bounds__(AS_THREADS) adapter_sort_kernel(const AhArgs g
   }
 }
 
-// grid (nt, tiles_n, slices): a CTA for 16 ranks of a row's slot, 8 columns per
-// thread and turn, summed over the threads at the end. The operations are few
-// (rows * rank * in); what counts is that the kernel ends while the head still
-// multiplies its first tile, so it is spread over as many CTAs as there are rows,
-// and leaves the SM room for the head beside it. Unsorted, every CTA lists its
-// tile's entries for itself, in the order of the slots.
+// grid (nt, tiles_n): a CTA for a row, its 16 ranks at a time, 8 columns per thread
+// and turn, summed over the threads at the end. The operations are few (rows * rank
+// * in); what counts is that the kernel ends while the head still multiplies its
+// first tile, so it is spread over as many CTAs as there are rows, four to an SM:
+// the head starts when all of them have. Unsorted (nt <= AH_SINGLE), every CTA
+// lists its tile's entries for itself, in the order of the slots.
 template <typename E, bool SORTED>
-__global__ void __launch_bounds__(AS_THREADS, 2) adapter_shrink_kernel(const AhArgs g) {
+__global__ void __launch_bounds__(AU_THREADS, 4) adapter_shrink_kernel(const AhArgs g) {
   // sorted: the head starts when every CTA is here, and so after the sort's end
   if constexpr (SORTED) asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
-  __shared__ uint32_t taken[AH_MAX_ADAPTERS / 4];  // a byte per slot: its entries, once named
-  __shared__ int32_t first[AH_MAX_ADAPTERS];       // and the first of them
-  __shared__ int32_t warp_sum[AS_THREADS / 32];
-  __shared__ float part[AS_THREADS / 32][16];
+  __shared__ int32_t key[AH_SINGLE];  // slot << 8 | entries of each row, the largest number for none
+  __shared__ float part[AU_THREADS / 32][16];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const int r = blockIdx.x, tile = blockIdx.y, slice = blockIdx.z, n0 = tile * g.nt;
-  int mine, used = 0;
+  const int r = blockIdx.x, tile = blockIdx.y, n0 = tile * g.nt;
+  int mine;
   const int slot = as_slot(g, n0 + r, &mine);
-  if (slice >= mine && (SORTED || slice > 0)) return;
-  int other = -1;
-  int4 info{};
-  if constexpr (SORTED) info = g.info[tile * AH_NT + r];
-  else if (t < g.nt) other = as_slot(g, n0 + t, &used);
-  taken[t] = 0;
-
-  float acc[16] = {};
-  if (mine) {
-    const E* a = static_cast<const E*>(g.a) + ((int64_t)slot * g.slices + slice) * 16 * (int64_t)g.kpad;
-    const E* x = SORTED ? static_cast<const E*>(g.x_sorted) + (int64_t)(n0 + info.x) * g.kpad
-                        : static_cast<const E*>(g.x) + (int64_t)(n0 + r) * g.ldx;
-    for (int k = t * 8; k < g.kpad; k += AS_THREADS * 8) {
-      const uint4 xv = ah_row8(x, k, g.in);
-      uint4 av[16];
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        av[j] = __ldg(reinterpret_cast<const uint4*>(a + (int64_t)j * g.kpad + k));
-      const float2 x0 = ah_pair<E>(xv.x), x1 = ah_pair<E>(xv.y), x2 = ah_pair<E>(xv.z),
-                   x3 = ah_pair<E>(xv.w);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float2 a0 = ah_pair<E>(av[j].x), a1 = ah_pair<E>(av[j].y), a2 = ah_pair<E>(av[j].z),
-                     a3 = ah_pair<E>(av[j].w);
-        acc[j] = fmaf(a0.x, x0.x, fmaf(a0.y, x0.y, acc[j]));
-        acc[j] = fmaf(a1.x, x1.x, fmaf(a1.y, x1.y, acc[j]));
-        acc[j] = fmaf(a2.x, x2.x, fmaf(a2.y, x2.y, acc[j]));
-        acc[j] = fmaf(a3.x, x3.x, fmaf(a3.y, x3.y, acc[j]));
+  E* u = static_cast<E*>(g.u) + (int64_t)tile * g.max_entries * 2 * g.block * 16;
+  // where an entry's part of the block's row `at` lies, hi; lo is bh rows further
+  auto row_of = [&](int e, int at) {
+    return u + ((int64_t)(at / g.bh) * g.max_entries + e) * 2 * g.bh * 16;
+  };
+  auto clear = [&](int e, int at, int quarter) {  // 16 bytes of the row's hi and lo
+    *reinterpret_cast<uint4*>(row_of(e, at) + (quarter & 2 ? g.bh * 16 : 0) + at % g.bh * 16 +
+                              (quarter & 1) * 8) = make_uint4(0, 0, 0, 0);
+  };
+  int own, next, place;  // the row's first entry, how far to the next 16 ranks', the row in it
+  const E* x = static_cast<const E*>(g.x) + (int64_t)(n0 + r) * g.ldx;
+  if constexpr (SORTED) {
+    if (!mine) return;
+    const int4 info = g.info[tile * AH_NT + r];
+    const int b0 = info.z / AH_BLOCK, b1 = info.w / AH_BLOCK;
+    next = b1 - b0 + 1;
+    own = info.y + info.x / AH_BLOCK - b0;
+    place = info.x % AH_BLOCK;
+    x = static_cast<const E*>(g.x_sorted) + (int64_t)(n0 + info.x) * g.kpad;
+    if (info.x == info.z)  // the slot's first row clears what is not the slot's
+      for (int j = 0; j < mine; ++j) {
+        const int front = info.z % AH_BLOCK, back = AH_BLOCK - 1 - info.w % AH_BLOCK;
+        const int e = info.y + j * next;
+        for (int i = t; i < 4 * front; i += AU_THREADS) clear(e, i >> 2, i & 3);
+        for (int i = t; i < 4 * back; i += AU_THREADS)
+          clear(e + b1 - b0, AH_BLOCK - back + (i >> 2), i & 3);
       }
+  } else {
+    const int none = 0x7FFFFFFF;
+    int kt = none;
+    if (t < g.nt) {
+      int n;
+      const int s = as_slot(g, n0 + t, &n);
+      if (s >= 0) kt = s << 8 | n;
+      key[t] = kt;
+    }
+    __syncthreads();
+    bool leads = kt != none;  // the slot's first row speaks for it
+    for (int i = 0; leads && i < t; ++i) leads = key[i] != kt;
+    __syncthreads();
+    if (t < g.nt && !leads) key[t] = none;
+    __syncthreads();
+    // a slot's entries are behind those of all lower slots
+    const int k = mine ? slot << 8 | mine : none;
+    int before = 0, count = 0, mine_at = 0;
+    for (int i = 0; i < g.nt; ++i) {
+      const int ki = key[i], n = ki == none ? 0 : ki & 255;
+      count += n;
+      before += ki < k ? n : 0;
+      mine_at += ki < kt ? n : 0;
+    }
+    own = before;
+    next = 1;
+    place = r;
+    if (r == 0) {  // row 0's CTA writes the list down
+      int2* entries = g.entries + (int64_t)tile * g.max_entries;
+      if (leads)
+        for (int i = 0; i < (kt & 255); ++i)
+          entries[mine_at + i] = make_int2((kt >> 8) * g.slices + i, 0);
+      if (t == 0) g.counts[tile] = count;
+    }
+    for (int i = t; i < 4 * count; i += AU_THREADS)
+      if (i >> 2 < own || i >> 2 >= own + mine) clear(i >> 2, r, i & 3);
+    if (!mine) return;
+  }
+  for (int slice = 0; slice < mine; ++slice) {
+  float acc[16] = {};
+  const E* a = static_cast<const E*>(g.a) + ((int64_t)slot * g.slices + slice) * 16 * (int64_t)g.kpad;
+  for (int k = t * 8; k < g.kpad; k += AU_THREADS * 8) {
+    const uint4 xv = ah_row8(x, k, g.in);
+    uint4 av[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      av[j] = __ldg(reinterpret_cast<const uint4*>(a + (int64_t)j * g.kpad + k));
+    const float2 x0 = ah_pair<E>(xv.x), x1 = ah_pair<E>(xv.y), x2 = ah_pair<E>(xv.z),
+                 x3 = ah_pair<E>(xv.w);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float2 a0 = ah_pair<E>(av[j].x), a1 = ah_pair<E>(av[j].y), a2 = ah_pair<E>(av[j].z),
+                   a3 = ah_pair<E>(av[j].w);
+      acc[j] = fmaf(a0.x, x0.x, fmaf(a0.y, x0.y, acc[j]));
+      acc[j] = fmaf(a1.x, x1.x, fmaf(a1.y, x1.y, acc[j]));
+      acc[j] = fmaf(a2.x, x2.x, fmaf(a2.y, x2.y, acc[j]));
+      acc[j] = fmaf(a3.x, x3.x, fmaf(a3.y, x3.y, acc[j]));
     }
   }
   // sums over the warp: lane l ends with those of rank l / 2
@@ -305,62 +361,19 @@ __global__ void __launch_bounds__(AS_THREADS, 2) adapter_shrink_kernel(const AhA
   if ((lane & 1) == 0) part[warp][lane >> 1] = acc[0];
   __syncthreads();
 
-  E* u = static_cast<E*>(g.u) + (int64_t)tile * g.max_entries * 2 * g.block * 16;
-  // where row `at` of an entry's block lies, hi; lo is bh rows further
-  auto row_of = [&](int e, int at) {
-    return u + ((int64_t)e * 2 * g.block + at / g.bh * 2 * g.bh) * 16;
-  };
-  auto clear = [&](int e, int at, int quarter) {  // 16 bytes of the row's hi and lo
-    *reinterpret_cast<uint4*>(row_of(e, at) + (quarter & 2 ? g.bh * 16 : 0) + at % g.bh * 16 +
-                              (quarter & 1) * 8) = make_uint4(0, 0, 0, 0);
-  };
-  int own, place;  // the entry this CTA writes into, the row of it
-  if constexpr (SORTED) {
-    const int b0 = info.z / AH_BLOCK, b1 = info.w / AH_BLOCK, e0 = info.y + slice * (b1 - b0 + 1);
-    own = e0 + info.x / AH_BLOCK - b0;
-    place = info.x % AH_BLOCK;
-    if (info.x == info.z) {  // the slot's first row clears what is not the slot's
-      const int front = info.z % AH_BLOCK, back = AH_BLOCK - 1 - info.w % AH_BLOCK;
-      for (int i = t; i < 4 * front; i += AS_THREADS) clear(e0, i >> 2, i & 3);
-      for (int i = t; i < 4 * back; i += AS_THREADS)
-        clear(e0 + b1 - b0, AH_BLOCK - back + (i >> 2), i & 3);
-    }
-  } else {
-    if (used) reinterpret_cast<uint8_t*>(taken)[other] = (uint8_t)used;  // equal for equal slots
-    __syncthreads();
-    const uint32_t four = taken[t];
-    const int c0 = four & 255, c1 = four >> 8 & 255, c2 = four >> 16 & 255, c3 = four >> 24;
-    int count;
-    const int at = as_scan(c0 + c1 + c2 + c3, warp_sum, &count);
-    first[4 * t] = at;
-    first[4 * t + 1] = at + c0;
-    first[4 * t + 2] = at + c0 + c1;
-    first[4 * t + 3] = at + c0 + c1 + c2;
-    if (r == 0 && slice == 0) {  // row 0's CTA writes the list down
-      int2* entries = g.entries + (int64_t)tile * g.max_entries;
-      for (int j = 0, e = at; j < 4; ++j)
-        for (int i = 0; i < (int)(four >> (8 * j) & 255); ++i)
-          entries[e++] = make_int2((4 * t + j) * g.slices + i, 0);
-      if (t == 0) g.counts[tile] = count;
-    }
-    __syncthreads();
-    own = (mine ? first[slot] : 0) + slice;
-    place = r;
-    if (slice == 0)
-      for (int i = t; i < 4 * count; i += AS_THREADS)
-        if (i >> 2 < own || i >> 2 >= own + mine) clear(i >> 2, r, i & 3);
-  }
-  if (mine && t < 16) {
+  if (t < 16) {
     float v = 0.0f;
 #pragma unroll
-    for (int w = 0; w < AS_THREADS / 32; ++w) v += part[w][t];
+    for (int w = 0; w < AU_THREADS / 32; ++w) v += part[w][t];
     v *= g.scales[slot];
     if (g.ranks[slot] < 0) v = NAN;
     const E hi = E(v);
     const E lo = E(fabsf((float)hi) < INFINITY ? v - (float)hi : 0.0f);
-    E* to = row_of(own, place) + ah_at(place % g.bh, t);
+    E* to = row_of(own + slice * next, place) + ah_at(place % g.bh, t);
     to[0] = hi;
     to[(int64_t)g.bh * 16] = lo;
+  }
+  __syncthreads();
   }
 }
 
@@ -487,7 +500,11 @@ __device__ __forceinline__ void ah_load16(uint32_t addr, uint32_t* r) {
 //
 // The outputs are dealt out evenly: every CTA takes g.share of them, a multiple of
 // 16, in tiles of 128 and a last, lower one, so that all read the same number of
-// weight bytes (whole tiles would leave a sixth of the SMs idle at 250 tiles).
+// weight bytes (whole tiles would leave a sixth of the SMs idle at 250 tiles). With
+// several tiles of rows, neighbouring CTAs (or pairs) work on the same outputs with
+// different ones of them, g.groups at a time, so that one reads from L2 what the
+// other brought there: 148 CTAs' tiles of 1 MB would not stay in L2 until a CTA
+// comes back to them (512x4096x75776 read its weight twice).
 //
 // CPT > 0 (fp32 output): the sum over the inner axis is cut into pieces of
 // AH_PIECE stages, each summed in TMEM from zero and added up in registers, CPT
@@ -546,19 +563,21 @@ __global__ void __launch_bounds__(AH_THREADS, 1)
   ah_all_sync<CG>();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = s_tmem;
-  constexpr int PER = CG == 1 ? 2 : 4;  // entries per stage
+  constexpr int PER = ah_per(CG);
   const int steps = (g.in + AH_BK - 1) / AH_BK;
   const int piece = CPT ? AH_PIECE : steps;  // stages added up in TMEM
   const int pieces = (steps + piece - 1) / piece;
-  const int v_begin = blockIdx.x * g.share, tiles_m = (g.share + AH_BM - 1) / AH_BM;
+  const int at = blockIdx.x / CG, group = at % g.groups;
+  const int v_begin = (at / g.groups * CG + rank) * g.share, tiles_m = (g.share + AH_BM - 1) / AH_BM;
+  const int tiles_n = (g.tiles_n - group + g.groups - 1) / g.groups;  // this CTA's
 
   if (warp == AH_EPILOGUE) {  // ---- copies: the warp waits together, a lane issues ------------
     int s = 0, issued = 0;
     uint32_t phase = 0;
     bool ok = true, waited = false;
     if (g.order) asm volatile("fence.proxy.async.global;" ::: "memory");  // the sorted x
-    for (int i = 0; ok && i < tiles_m * g.tiles_n; ++i) {
-      const int m = i / g.tiles_n, n = i % g.tiles_n;
+    for (int i = 0; ok && i < tiles_m * tiles_n; ++i) {
+      const int m = i / tiles_n, n = group + i % tiles_n * g.groups;
       const int v0 = v_begin + m * AH_BM, high = min(AH_BM, g.share - m * AH_BM);
       const int2* entries = g.entries + (int64_t)n * g.max_entries;
       int count = 0;  // entries of the tile of rows; lane l holds the l-th of 32
@@ -594,14 +613,15 @@ __global__ void __launch_bounds__(AH_THREADS, 1)
         if (!(ok = ah_wait(empty + 8 * s, phase ^ 1))) break;
         const int several = min(PER, count - e);
         const uint32_t a = stage0 + s * stage_bytes, bar = full + 8 * s;
-        if (lane == 0 && rank == 0) ah_expect(bar, CG * several * (AH_BM * 32 + g.bh * 64));
+        if (lane == 0) {  // U of a whole stage at once, whether it is full or not
+          if (rank == 0) ah_expect(bar, CG * (several * AH_BM * 32 + PER * g.bh * 64));
+          ah_copy<CG>(a + AH_A_BYTES, &map_u, bar, 0,
+                      (int)(((int64_t)(n * CG + rank) * g.max_entries + e) * g.bh / 8));
+        }
         for (int j = 0; j < several; ++j) {
           const int z = __shfl_sync(0xffffffffu, mine.x, (e & 31) + j);
-          if (lane == 0) {
+          if (lane == 0)
             ah_copy<CG>(a + j * AH_BM * 32, &map_b, bar, 0, (int)(((int64_t)z * g.opad + v0) / 16));
-            ah_copy<CG>(a + AH_A_BYTES + j * g.bh * 64, &map_u, bar, 0,
-                        (int)((((int64_t)n * g.max_entries + e + j) * 2 * g.block + rank * 2 * g.bh) / 16));
-          }
         }
         __syncwarp();
         ++issued;
@@ -621,8 +641,8 @@ __global__ void __launch_bounds__(AH_THREADS, 1)
       int s = 0, turn = 0;
       uint32_t phase = 0;
       bool ok = true, waited = false;
-      for (int i = 0; ok && i < tiles_m * g.tiles_n; ++i) {
-        const int n = i % g.tiles_n;
+      for (int i = 0; ok && i < tiles_m * tiles_n; ++i) {
+        const int n = group + i % tiles_n * g.groups;
         const int2* entries = g.entries + (int64_t)n * g.max_entries;
         int count = 0, mine = 0;  // as above; of an entry, the first place of its block
         if (waited && g.ids) {
@@ -699,13 +719,13 @@ __global__ void __launch_bounds__(AH_THREADS, 1)
     O* y = static_cast<O*>(g.y);
     const int half = (g.nt / 2 + 15) / 16 * 16, c_begin = (warp >> 2) * half,
               c_end = min(g.nt, c_begin + half);
-    for (int i = 0; ok && i < tiles_m * g.tiles_n; ++i) {
-      const int m = i / g.tiles_n, n0 = i % g.tiles_n * g.nt;
+    for (int i = 0; ok && i < tiles_m * tiles_n; ++i) {
+      const int m = i / tiles_n, n = group + i % tiles_n * g.groups, n0 = n * g.nt;
       const int in_tile = (warp & 3) * 32 + lane, v = v_begin + m * AH_BM + in_tile;
       const bool store = v < g.out && m * AH_BM + in_tile < g.share;
       const int here = min(c_end, g.rows - n0);  // columns with a row behind them end here
       O* to = y + (int64_t)n0 * g.ldo + v;
-      const int32_t* order = g.order + i % g.tiles_n * AH_NT;
+      const int32_t* order = g.order + n * AH_NT;
       auto put = [&](int c, float x) {  // the row in place c of the tile
         if (c < here) to[(int64_t)(g.order ? order[c] : c) * g.ldo] = O(x);
       };
@@ -783,6 +803,8 @@ struct NcbAdapterHead {
   uint32_t* error_word = nullptr;
   void* w_own = nullptr;  // the weight's copy, where it cannot be read in place
   bool has_w = false;
+  const void* w = nullptr;  // what is read: the caller's weight or the copy
+  int64_t ldw = 0;
   CUtensorMap map_w{}, map_low{}, map_b{};  // map_low: a CTA's last, lower tile
 };
 
@@ -853,6 +875,8 @@ void ah_align(void* to, int64_t pitch, const void* from, int64_t ld, int64_t row
       static_cast<uint16_t*>(to), pitch, static_cast<const uint16_t*>(from), ld, rows, cols);
 }
 
+constexpr int64_t AH_L2 = 64ll << 20;  // of 126 MB: what weight tiles may take of it
+
 struct AhMaps {
   CUtensorMap w, low, x, b, u;
 };
@@ -880,8 +904,8 @@ bool ah_start(void (*kernel)(A...), dim3 grid, int threads, size_t smem, int clu
 
 template <typename O, int CG, int CPT>
 bool ah_launch(const AhMaps& m, const nvs::AhArgs& g, cudaStream_t st) {
-  const int ctas = (g.out + g.share - 1) / g.share;
-  return ah_start(nvs::head_kernel<O, CG, CPT>, dim3((ctas + CG - 1) / CG * CG), nvs::AH_THREADS,
+  const int units = ((g.out + g.share - 1) / g.share + CG - 1) / CG;  // CTAs or pairs with outputs
+  return ah_start(nvs::head_kernel<O, CG, CPT>, dim3(units * g.groups * CG), nvs::AH_THREADS,
                   (size_t)g.stages * (nvs::AH_A_BYTES + g.nh * 128) + 1024, CG, g.ids != nullptr, st,
                   m.w, m.low, m.x, m.b, m.u, g);
 }
@@ -889,10 +913,10 @@ template <typename E, int CG>
 int ah_head(const AhMaps& m, const nvs::AhArgs& g, bool wide, cudaStream_t st) {
   bool ok = true;
   if (g.ids) {
-    const dim3 grid(g.nt, g.tiles_n, g.slices);
+    const dim3 grid(g.nt, g.tiles_n);
     if constexpr (CG == 2)
-      ok = ah_start(nvs::adapter_sort_kernel, dim3(g.nt, g.tiles_n), nvs::AS_THREADS, 0, 1, false, st, g);
-    ok = ok && ah_start(nvs::adapter_shrink_kernel<E, CG == 2>, grid, nvs::AS_THREADS, 0, 1, CG == 2, st, g);
+      ok = ah_start(nvs::adapter_sort_kernel, grid, nvs::AS_THREADS, 0, 1, false, st, g);
+    ok = ok && ah_start(nvs::adapter_shrink_kernel<E, CG == 2>, grid, nvs::AU_THREADS, 0, 1, CG == 2, st, g);
   }
   // fp32 sums stay in registers: those of half of the tile's rows per thread
   if (!wide) ok = ok && ah_launch<E, CG, 0>(m, g, st);
@@ -1047,6 +1071,8 @@ NCB_API int ncb_adapter_head_set_weight_device(NcbAdapterHead* h, const void* d_
     d_weight = h->w_own;
     ld = h->kpad;
   }
+  h->w = d_weight;
+  h->ldw = ld;
   h->has_w = ah_map(&h->map_w, h->dtype, d_weight, h->in, h->out, ld, nvs::AH_BK, nvs::AH_BM,
                      CU_TENSOR_MAP_SWIZZLE_128B) &&
              ah_map(&h->map_low, h->dtype, d_weight, h->in, h->out, ld, nvs::AH_BK,
@@ -1137,7 +1163,23 @@ NCB_API int ncb_adapter_head_project_device(NcbAdapterHead* h, const void* d_x, 
   g.idesc_u = kind | (uint32_t)(g.block / 8) << 17;
   const int stage = nvs::AH_A_BYTES + g.nh * 128;
   g.stages = nvs::AH_SMEM / stage < nvs::AH_MAX_STAGES ? nvs::AH_SMEM / stage : nvs::AH_MAX_STAGES;
+  // Tiles of rows at the same time: as many as take the fewest turns (tiles of
+  // outputs times tiles of rows, of one CTA), among those whose weight tiles stay in
+  // L2 until the CTA comes back to them, or that come back to none.
   g.share = h->share;
+  g.groups = 1;
+  int64_t turns = INT64_MAX;
+  for (int n = 1; n <= g.tiles_n && n <= 8; ++n) {
+    const int ctas = h->num_sms / group / n * group;
+    const int share = ((h->out + ctas - 1) / ctas + 15) / 16 * 16;
+    const int64_t live = (int64_t)ctas * nvs::AH_BM * h->kpad * 2;
+    const int64_t t = (int64_t)((share + nvs::AH_BM - 1) / nvs::AH_BM) * ((g.tiles_n + n - 1) / n);
+    if (t <= turns && (n == g.tiles_n || n == 8 || live <= AH_L2)) {
+      turns = t;
+      g.groups = n;
+      g.share = share;
+    }
+  }
   g.error_word = h->error_word;
   if (!sorted && !ah_readable(d_x, ldx)) {  // (the sort copies x anyway)
     ah_align(h->x_own, h->kpad, d_x, ldx, rows, h->in, h->num_sms, st);
@@ -1147,10 +1189,14 @@ NCB_API int ncb_adapter_head_project_device(NcbAdapterHead* h, const void* d_x, 
   g.x = d_x;
   g.ldx = ldx;
   AhMaps m{h->map_w, h->map_low, {}, h->map_b, h->map_w};
+  if (g.share != h->share &&
+      !ah_map(&m.low, h->dtype, h->w, h->in, h->out, h->ldw, nvs::AH_BK, (g.share - 1) % nvs::AH_BM + 1,
+              CU_TENSOR_MAP_SWIZZLE_128B))
+    return ncb_record_status(NCB_ERROR_LAUNCH_FAILED);
   if (!ah_map(&m.x, h->dtype, sorted ? h->x_own : d_x, h->in, rows, sorted ? h->kpad : ldx,
               nvs::AH_BK, g.nh, CU_TENSOR_MAP_SWIZZLE_128B) ||
       (g.ids && !ah_map(&m.u, h->dtype, h->u, 256, (int64_t)g.tiles_n * g.max_entries * 2 * g.block / 16,
-                        256, 256, g.bh / 8, CU_TENSOR_MAP_SWIZZLE_NONE)))
+                        256, 256, nvs::ah_per(group) * g.bh / 8, CU_TENSOR_MAP_SWIZZLE_NONE)))
     return ncb_record_status(NCB_ERROR_LAUNCH_FAILED);
   const bool wide = out_dtype == NCB_DTYPE_F32;
   if (h->dtype == NCB_DTYPE_BF16)

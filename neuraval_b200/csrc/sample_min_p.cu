@@ -7,24 +7,29 @@
 //
 // Every set is a prefix of the order, so a row needs no sort, only the places
 // where a count (top_k), a value (min_p) or a mass (top_p, the draw) is crossed.
-// A row belongs to a cluster of 1..8 CTAs, each holding its slice of the row in
-// shared memory, so that the row is read from HBM once. CTA 0 decides, the
+// A row belongs to a cluster of 1..8 CTAs (more CTAs for few rows), which pass over
+// it two or three times; all passes but the first mostly read L2. CTA 0 decides, the
 // others carry out its commands:
-//   1. load the slice, maximum and least finite value (NaN and +inf show in a
-//      NaN-propagating maximum);
-//   2. histogram of counts over SP_BINS equal steps of x below the maximum
-//      (counts are integers: their order does not matter). From the counts CTA 0
-//      knows the bin of the k-th value exactly, and with n_b exp(centre) about
-//      where the masses are crossed;
-//   3. few values wanted (the usual options): those bins are gathered into one
-//      list, sorted by (x, id), and everything is decided on 64-bit prefix sums
-//      of the list. Many: one pass sums the exact 64-bit weights above each
-//      guessed window of bins and gathers the windows; a crossing outside its
-//      window moves the window and repeats the pass, a window with more values
-//      than a list holds is divided by a histogram of the value's bits, down to
-//      a single value, whose crossing is a division.
+//   1. maximum and least finite value (NaN and +inf show in a NaN-propagating
+//      maximum), and each thread's own maximum;
+//   2. few values wanted (the usual options): the k-th largest of the threads'
+//      maxima is a lower bound of the k-th value, min-p has one of its own. What is
+//      above is gathered into one list, sorted by (x, id), and everything is decided
+//      on 64-bit prefix sums of the list.
+//   3. Otherwise, or where the list overflows: a histogram of counts over SP_BINS
+//      equal steps of x below the maximum (integers: their order does not matter).
+//      It gives the bin of the k-th value exactly, and about where the masses are
+//      crossed. One more pass sums the exact 64-bit weights above each guessed
+//      window of bins and gathers the windows; a crossing outside its window moves
+//      the window and repeats the pass; a window with more values than a list holds
+//      is one value many times, whose crossing is a division, or is divided by a
+//      histogram of the values' bits.
 // Sums run in an order fixed by the sizes alone; the lists' order of arrival is
 // sorted away.
+//
+// Keeping a cluster's slices of the row in shared memory, for one read in all, was
+// slower: it leaves two CTAs per SM in long chains of small steps, and more of them
+// per row to synchronise (1024x151936: 2.3 ms, now NOWFLAT).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -44,8 +49,11 @@ namespace cg = cooperative_groups;
 
 constexpr int SP_NT = 512;       // threads of a CTA
 constexpr int SP_BINS = 2048;    // histogram bins (four per thread)
-constexpr int SP_LIST = 2048;    // places of the gather list
-constexpr int SP_CAP = 512;      // places of one window's part of it
+constexpr int SP_FEW = 1024;     // values that one list holds and sorts
+constexpr int SP_CAP = 512;      // and one window's part of the list
+constexpr int SP_WIDEN = 96;     // values up to which a guessed window takes in its neighbours
+constexpr int SP_RANKED = 256;   // lists up to this are sorted by ranks
+constexpr int SP_BOUNDED = 256;  // largest top_k that the threads' maxima bound
 constexpr int SP_CLUSTER = 8;    // largest cluster
 constexpr int SP_TURNS = 4096;   // passes over a row at most
 constexpr int SP_MAX_VOCAB = 1 << 24;
@@ -70,16 +78,16 @@ struct SpArgs {
   uint32_t* flags;
 };
 
-enum { SP_DONE = 0, SP_PASS = 1, SP_HIST = 2, SP_GATHER = 3, SP_SELECT = 4 };
+enum { SP_DONE, SP_FIRST, SP_PASS, SP_HIST, SP_GATHER, SP_SELECT };
 enum { SP_K = 0, SP_P = 1, SP_D = 2, SP_WINDOWS = 3 };
 
 struct SpCmd {
   int op;
+  float above[SP_WINDOWS], below[SP_WINDOWS];  // SP_FIRST: each window's bins, [above, below)
   uint32_t klo[SP_WINDOWS], khi[SP_WINDOWS];  // each window's keys, both ends in it
   int gather[SP_WINDOWS];                     // whether its values are listed
   float theta;                                // least value that min-p keeps
   int shift;                                  // SP_HIST: bin = (khi[0] - key) >> shift; < 0: bin(value)
-  int bin;                                    // SP_GATHER: bins up to this one
   float value;                                // SP_SELECT: the value and which of its
   int nth;                                    //   occurrences, by id
 };
@@ -98,14 +106,15 @@ struct SpPart {
 
 struct SpShared {
   uint4 hist4[SP_BINS / 4];  // counts; in CTA 0, once merged, the counts before each bin
-  float mass[SP_BINS + 4];   // CTA 0: about the mass before each bin
-  unsigned long long list[SP_LIST];
-  double table[256];         // 2^(j/256)
+  float4 some4[SP_BINS / 4]; // a value of each filled bin
+  alignas(16) float mass[SP_BINS + 4];  // CTA 0, once merged: about the mass before each bin
+  unsigned long long list[SP_WINDOWS * SP_CAP];
   SpCmd cmd;
   SpPart part[SP_CLUSTER];
   float mx[SP_CLUSTER], mn[SP_CLUSTER];
   int count[SP_CLUSTER];
   int n_list[SP_WINDOWS];
+  uint32_t k_low[SP_CLUSTER][SP_WINDOWS], k_high[SP_CLUSTER][SP_WINDOWS];  // least and greatest key in a window
   int token;
   int total;  // finite values of the row
   // scratch of the block-wide steps
@@ -114,9 +123,15 @@ struct SpShared {
   int red_i[SP_NT / 32];
   SpPart warp_part[SP_NT / 32];
   double got_d;
-  int got_i;
-  uint32_t tops[8];
+  int got_i, bin_k, bin_last;
+  float theta;
+  uint32_t tops[2];
 };
+
+// The CTA's shared memory, by a name that is known to be shared: through a pointer in
+// SpRow every access would be a generic one.
+extern __shared__ uint4 sp_raw[];
+__device__ __forceinline__ SpShared& sp_shared() { return *reinterpret_cast<SpShared*>(sp_raw); }
 
 // Floats in order as unsigned integers; -0 counts as +0.
 __device__ __forceinline__ uint32_t sp_key(float v) {
@@ -177,19 +192,17 @@ struct SpVec<__half> {
 // the 16-byte boundary at or below the row's first value. Only the row's first and
 // last granule can hold values of other rows; they are read value by value and
 // filled up with -inf.
-template <typename E, bool RES>
+template <typename E>
 struct SpSlice {
   const char* base;  // the row's first granule
   int skip;          // values of granule 0 before the row's first
   int vocab, g0, n;
-  uint4* sm;
 
-  __device__ __forceinline__ uint4 fetch(int i) const {
+  // Granule i of the slice, whole or not.
+  __device__ __noinline__ uint4 fetch(int i) const {
     constexpr int N = SpVec<E>::N;
-    const int g = g0 + i;
-    const int first = g * N - skip;
-    if (first >= 0 && first + N <= vocab)
-      return __ldcs(reinterpret_cast<const uint4*>(base) + g);
+    const int g = g0 + i, first = g * N - skip;
+    if (first >= 0 && first + N <= vocab) return __ldg(reinterpret_cast<const uint4*>(base) + g);
     uint32_t w[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -213,33 +226,63 @@ struct SpSlice {
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
-  __device__ __forceinline__ uint4 again(int i) const {
-    if constexpr (RES) return sm[i];
-    return fetch(i);
+  // f(values, granule) for this thread's granules, FLIGHT loads at a time. The whole
+  // granules are read without a branch (the loads would wait for one another); past
+  // the end the last one is read again and dropped.
+  template <int FLIGHT, typename F>
+  __device__ __forceinline__ void each(F f) const {
+    constexpr int N = SpVec<E>::N;
+    const int lo = n > 0 && g0 * N < skip ? 1 : 0;
+    const int hi = n > lo && (g0 + n) * N - skip > vocab ? n - 1 : n;
+    const uint4* from = reinterpret_cast<const uint4*>(base) + g0;
+    uint4 g[FLIGHT];
+    auto load = [&](int i0) {
+#pragma unroll
+      for (int j = 0; j < FLIGHT; ++j) g[j] = __ldg(from + min(i0 + j * SP_NT, hi - 1));
+    };
+    const int i0 = lo + threadIdx.x;
+    if (lo < hi) load(i0);
+#pragma unroll 1
+    for (int i = i0; i < hi; i += FLIGHT * SP_NT) {
+      uint4 now[FLIGHT];
+#pragma unroll
+      for (int j = 0; j < FLIGHT; ++j) now[j] = g[j];
+      load(i + FLIGHT * SP_NT);  // on its way while f works
+#pragma unroll
+      for (int j = 0; j < FLIGHT; ++j)
+        if (i + j * SP_NT < hi) {
+          float v[N];
+          SpVec<E>::get(now[j], v);
+          f(v, i + j * SP_NT);
+        }
+    }
+    const int edge = threadIdx.x == 0 && lo ? 0 : threadIdx.x == 32 && hi < n ? n - 1 : -1;
+    if (edge >= 0) {
+      float v[N];
+      SpVec<E>::get(fetch(edge), v);
+      f(v, edge);
+    }
   }
   __device__ __forceinline__ int id(int i, int e) const {
     return (g0 + i) * SpVec<E>::N - skip + e;
   }
 };
 
-// exp(d c ln2 / 256) for 0 >= d c > -2^20: with d c = n + r, n whole, |r| <= 1/2,
-// it is 2^(n / 256) (a table of 2^(j/256) and an exponent) times exp(r ln2 / 256),
-// whose series needs four terms for 2^-53. Own code: 64-bit library exponentials
-// take about twice the instructions, and a pass over a row is bound by them.
-__device__ __forceinline__ double sp_exp(const double* table, double d, double c) {
+// exp(d c ln2) for 0 >= d c > -1000: with d c = n + r, n whole, |r| <= 1/2, it is 2^n
+// times the series of exp(r ln2), cut off after r^11 (6e-15 of it). Own code, for the
+// range that is needed: a pass over a row is bound by these operations. (A table of
+// 1024 values and three terms took as long: random reads of shared memory.)
+__device__ __forceinline__ double sp_exp(double d, double c) {
   const double magic = 6755399441055744.0;  // 1.5 * 2^52: rounds to a whole number
-  constexpr double l = 0.69314718055994530942 / 256.0;
-  const double m = d * c;
-  const double t = m + magic;
-  const double r = m - (t - magic);
-  const int n = __double2loint(t);
-  const double s = table[n & 255];
-  double q = fma(r, l * l * l * l / 24.0, l * l * l / 6.0);
-  q = fma(q, r, l * l / 2.0);
-  q = fma(q, r, l);
-  q = q * r;
-  const double w = fma(s, q, s);
-  return __hiloint2double(__double2hiint(w) + ((n >> 8) << 20), __double2loint(w));
+  constexpr double l = 0.69314718055994530942, l2 = l * l, l4 = l2 * l2, l8 = l4 * l4;
+  const double t = fma(d, c, magic);
+  const double r = fma(d, c, magic - t), r2 = r * r, r4 = r2 * r2;
+  const double a = fma(r, l, 1.0), b = fma(r, l2 * l / 6.0, l2 / 2.0),
+               e = fma(r, l4 * l / 120.0, l4 / 24.0), f = fma(r, l4 * l2 * l / 5040.0, l4 * l2 / 720.0),
+               g = fma(r, l8 * l / 362880.0, l8 / 40320.0),
+               h = fma(r, l8 * l2 * l / 39916800.0, l8 * l2 / 3628800.0);
+  const double w = fma(fma(fma(h, r2, g), r4, fma(f, r2, e)), r4, fma(b, r2, a));
+  return __hiloint2double(__double2hiint(w) + (__double2loint(t) << 20), __double2loint(w));
 }
 
 template <typename T>
@@ -279,17 +322,35 @@ __device__ __forceinline__ int sp_block_sum(int v, int* red) {
   return all;
 }
 
-// Bitonic sort, largest first; places [n, power of two) are filled with 0, which
-// no listed value has (its low half is never 0).
-__device__ void sp_sort(unsigned long long* list, int n) {
-  int p = 32;
+// Sorts a list, largest first. Short ones by their ranks: several threads count the
+// larger entries for each. Longer ones bitonically; places [n, power of two) are
+// filled with 0, which no listed value has (its low half is never 0).
+__device__ __noinline__ void sp_sort(unsigned long long* list, int n) {
+  if (n <= SP_RANKED) {
+    const int log = n <= 64 ? 3 : n <= 128 ? 2 : 1, per = 1 << log;  // threads per entry
+    const int i = threadIdx.x >> log, part = threadIdx.x & (per - 1);
+    unsigned long long mine = 0;
+    int rank = 0;
+    if (i < n) {
+      mine = list[i];
+      for (int j = part; j < n; j += per) rank += list[j] > mine;
+    }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1)
+      if (o < per) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    __syncthreads();
+    if (i < n && part == 0) list[rank] = mine;
+    __syncthreads();
+    return;
+  }
+  int p = 2 * SP_RANKED;
   while (p < n) p <<= 1;
   for (int i = n + threadIdx.x; i < p; i += SP_NT) list[i] = 0;
   __syncthreads();
   for (int size = 2; size <= p; size <<= 1)
     for (int step = size >> 1; step > 0; step >>= 1) {
       for (int i = threadIdx.x; i < p / 2; i += SP_NT) {
-        const int lo = 2 * step * (i / step) + i % step, hi = lo + step;
+        const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
         const bool down = (lo & size) == 0;
         const unsigned long long x = list[lo], y = list[hi];
         if ((x < y) == down) {
@@ -301,68 +362,188 @@ __device__ void sp_sort(unsigned long long* list, int n) {
     }
 }
 
-template <typename E, bool RES>
-struct SpRow {
-  SpShared& s;
-  SpSlice<E, RES> sl;
-  cg::cluster_group cl;
-  int rank, ranks;
+__device__ void sp_write(const SpArgs& a, int row, int token, float logprob, int kept,
+                         uint32_t flags) {
+  a.tokens[row] = token;
+  if (a.logprobs) a.logprobs[row] = logprob;
+  if (a.kept) a.kept[row] = kept;
+  if (a.flags) a.flags[row] = flags;
+}
+
+// What a value of the row means. The passes work on a copy of their own: behind a
+// pointer, every store to shared memory would have it read again.
+struct SpView {
   float mx;           // the row's maximum
-  double c;           // 256 / (T ln 2)
+  double c;           // 1 / (T ln 2)
   double inv_t;
   float scale;        // bins per unit of x
   float zero;         // values below carry no mass (SP_REACH)
 
+  // A value's place among the bins; its whole part is the bin, the last bin has all
+  // further places.
+  __device__ __forceinline__ float place(float v) const {  // (finite: what is below INFINITY)
+    return fminf((mx - v) * scale, FLT_MAX);
+  }
   __device__ __forceinline__ int bin(float v) const {
-    return min(SP_BINS - 1, __float2int_rd((mx - v) * scale));
+    return min(SP_BINS - 1, __float2int_rd(place(v)));
   }
   __device__ __forceinline__ double weight(float v) const {
-    return sp_exp(s.table, (double)v - (double)mx, c);
+    return sp_exp((double)v - (double)mx, c);
   }
-  // for listed values, which may lie beyond the reach
+  // of a listed value
   __device__ __forceinline__ double weight_any(float v) const {
-    return v < zero ? exp(((double)v - (double)mx) * inv_t) : weight(v);
+    return exp(((double)v - (double)mx) * inv_t);
   }
-  __device__ __forceinline__ SpShared& of(int r) { return *cl.map_shared_rank(&s, r); }
+};
+
+template <typename E>
+struct SpRow {
+  SpSlice<E> sl;
+  cg::cluster_group cl;
+  int rank, ranks;
+  SpView k;
+
+  __device__ __forceinline__ SpShared& of(int r) { return *cl.map_shared_rank(&sp_shared(), r); }
 
   // ---- the commands, carried out by every CTA of the cluster ------------------
-  __device__ void hist_by_value() {
-    for (int i = threadIdx.x; i < sl.n; i += SP_NT) {
-      float v[SpVec<E>::N];
-      SpVec<E>::get(sl.again(i), v);
+  __device__ __noinline__ void hist_by_value() {
+    SpShared& s = sp_shared();
+    const SpView k = this->k;
+    sl.template each<2>([&](const float* v, int) {
 #pragma unroll
       for (int e = 0; e < SpVec<E>::N; ++e)
-        if (v[e] > -INFINITY) atomicAdd(reinterpret_cast<int*>(s.hist4) + bin(v[e]), 1);
-    }
+        if (v[e] > -INFINITY) {
+          const int b = k.bin(v[e]);
+          atomicAdd(reinterpret_cast<int*>(s.hist4) + b, 1);
+          reinterpret_cast<float*>(s.some4)[b] = v[e];  // any of them, for the guess alone
+        }
+    });
   }
-  __device__ void hist_by_key(const SpCmd& m) {
-    for (int i = threadIdx.x; i < sl.n; i += SP_NT) {
-      float v[SpVec<E>::N];
-      SpVec<E>::get(sl.again(i), v);
+  __device__ __noinline__ void hist_by_key(const SpCmd& m) {
+    SpShared& s = sp_shared();
+    sl.template each<1>([&](const float* v, int) {
 #pragma unroll
       for (int e = 0; e < SpVec<E>::N; ++e) {
         const uint32_t k = sp_key(v[e]);
-        if (k >= m.klo[0] && k <= m.khi[0])
-          atomicAdd(reinterpret_cast<int*>(s.hist4) + ((m.khi[0] - k) >> m.shift), 1);
+        if (k >= m.klo[0] && k <= m.khi[0]) {
+          const uint32_t b = (m.khi[0] - k) >> m.shift;
+          atomicAdd(reinterpret_cast<int*>(s.hist4) + b, 1);
+          reinterpret_cast<float*>(s.some4)[b] = v[e];
+        }
       }
-    }
+    });
   }
   __device__ __forceinline__ void put(SpShared& to, int w, int base, int cap, float v, int id) {
+    SpShared& s = sp_shared();
     const int at = atomicAdd(&to.n_list[w], 1);
     if (at < cap)
       to.list[base + at] = ((unsigned long long)sp_key(v) << 32) | (0xFFFFFFFFu - (uint32_t)id);
   }
-  __device__ void gather(const SpCmd& m) {
+  __device__ __noinline__ void gather(const SpCmd& m) {
+    SpShared& s = sp_shared();
+    const SpView k = this->k;
     SpShared& to = of(0);
-    for (int i = threadIdx.x; i < sl.n; i += SP_NT) {
-      float v[SpVec<E>::N];
-      SpVec<E>::get(sl.again(i), v);
+    const float below = m.below[0];
+    sl.template each<2>([&](const float* v, int i) {
 #pragma unroll
       for (int e = 0; e < SpVec<E>::N; ++e)
-        if (v[e] > -INFINITY && bin(v[e]) <= m.bin) put(to, 0, 0, SP_LIST, v[e], sl.id(i, e));
-    }
+        if (k.place(v[e]) < below && v[e] > -INFINITY) put(to, 0, 0, SP_FEW, v[e], sl.id(i, e));
+    });
   }
-  __device__ void pass(const SpCmd& m) {
+  // The usual pass: windows that are runs of bins. Exact masses above each and of what
+  // min-p keeps; the values of a window into its list, or, where they are too many,
+  // their least and greatest key (they may all be one value).
+  __device__ __noinline__ void first_pass(const SpCmd& m) {
+    SpShared& s = sp_shared();
+    const SpView k = this->k;
+    SpShared& to = of(0);
+    float above[SP_WINDOWS], below[SP_WINDOWS];
+#pragma unroll
+    for (int w = 0; w < SP_WINDOWS; ++w) {
+      above[w] = m.above[w];
+      below[w] = m.below[w];
+    }
+    const float theta = m.theta;
+    double mass[SP_WINDOWS + 1] = {};
+    uint32_t low[SP_WINDOWS], high[SP_WINDOWS];
+#pragma unroll
+    for (int w = 0; w < SP_WINDOWS; ++w) low[w] = 0xFFFFFFFFu, high[w] = 0;
+    int n = 0;
+    sl.template each<1>([&](const float* v, int i) {
+#pragma unroll
+      for (int e = 0; e < SpVec<E>::N; ++e) {
+        const float x = v[e], q = k.place(x);
+        // out of reach: weighed as if just within it, and not added
+        const double wt = k.weight(fmaxf(x, k.zero));
+        const bool near = x >= k.zero;
+        bool in = false;
+#pragma unroll
+        for (int w = 0; w < SP_WINDOWS; ++w) {
+          if (near && q < above[w]) mass[w] += wt;
+          in |= q >= above[w] && q < below[w];
+        }
+        if (near && x >= theta) mass[SP_WINDOWS] += wt;
+        n += x >= theta;
+        if (in && x > -INFINITY) {
+#pragma unroll
+          for (int w = 0; w < SP_WINDOWS; ++w)
+            if (q >= above[w] && q < below[w]) {
+              if (m.gather[w]) {
+                put(to, w, w * SP_CAP, SP_CAP, x, sl.id(i, e));
+              } else {
+                low[w] = min(low[w], sp_key(x));
+                high[w] = max(high[w], sp_key(x));
+              }
+            }
+        }
+      }
+    });
+#pragma unroll
+    for (int j = 0; j <= SP_WINDOWS; ++j)
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mass[j] += __shfl_xor_sync(0xffffffffu, mass[j], o);
+    n = __reduce_add_sync(0xffffffffu, n);
+    const int warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int w = 0; w < SP_WINDOWS; ++w) {
+      low[w] = __reduce_min_sync(0xffffffffu, low[w]);
+      high[w] = __reduce_max_sync(0xffffffffu, high[w]);
+    }
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+      for (int j = 0; j <= SP_WINDOWS; ++j) s.warp_part[warp].mass[j] = mass[j];
+      s.warp_part[warp].n[SP_WINDOWS] = n;
+#pragma unroll
+      for (int w = 0; w < SP_WINDOWS; ++w) {
+        s.warp_part[warp].n[w] = (int)low[w];
+        s.warp_part[warp].n[SP_WINDOWS + 1 + w] = (int)high[w];
+      }
+    }
+    __syncthreads();
+    const int j = threadIdx.x & 31;
+    if (threadIdx.x <= SP_WINDOWS) {
+      double sum = 0.0;
+      for (int w = 0; w < SP_NT / 32; ++w) sum += s.warp_part[w].mass[j];
+      to.part[rank].mass[j] = sum;
+    } else if (warp == 1 && j < SP_SUMS) {
+      int sum = 0;
+      uint32_t least = 0xFFFFFFFFu, most = 0;
+      for (int w = 0; w < SP_NT / 32; ++w) {
+        const int x = s.warp_part[w].n[j];
+        sum += x;
+        least = min(least, (uint32_t)x);
+        most = max(most, (uint32_t)x);
+      }
+      if (j < SP_WINDOWS) to.k_low[rank][j] = least;
+      else if (j == SP_WINDOWS) to.part[rank].n[j] = sum;
+      else to.k_high[rank][j - SP_WINDOWS - 1] = most;
+    }
+    __syncthreads();
+  }
+  // Any windows, by their keys, with what lies in them; those that fit are listed.
+  __device__ __noinline__ void pass(const SpCmd& m) {
+    SpShared& s = sp_shared();
+    const SpView k = this->k;
     SpShared& to = of(0);
     float lo[SP_WINDOWS], hi[SP_WINDOWS];
 #pragma unroll
@@ -372,14 +553,12 @@ struct SpRow {
       hi[w] = sp_value(m.khi[w] == 0x7FFFFFFFu ? 0x7FFFFFFEu : m.khi[w]);
     }
     SpPart p{};
-    for (int i = threadIdx.x; i < sl.n; i += SP_NT) {
-      float v[SpVec<E>::N];
-      SpVec<E>::get(sl.again(i), v);
+    sl.template each<1>([&](const float* v, int i) {
 #pragma unroll
       for (int e = 0; e < SpVec<E>::N; ++e) {
         const float x = v[e];
         if (!(x > -INFINITY)) continue;
-        const double wt = x >= zero ? weight(x) : 0.0;
+        const double wt = x >= k.zero ? k.weight(x) : 0.0;
 #pragma unroll
         for (int w = 0; w < SP_WINDOWS; ++w) {
           if (x > hi[w]) {
@@ -396,7 +575,7 @@ struct SpRow {
           ++p.n[SP_WINDOWS];
         }
       }
-    }
+    });
 #pragma unroll
     for (int j = 0; j < SP_SUMS; ++j) {
 #pragma unroll
@@ -419,13 +598,14 @@ struct SpRow {
   }
   // The id of the nth occurrence of a value, counted over the CTAs in the order of
   // their slices and inside a CTA over its threads, each with granules in a row.
-  __device__ void select(const SpCmd& m) {
+  __device__ __noinline__ void select(const SpCmd& m) {
+    SpShared& s = sp_shared();
     const int q = (sl.n + SP_NT - 1) / SP_NT;
     const int b = min(sl.n, (int)threadIdx.x * q), e = min(sl.n, b + q);
     int mine = 0;
     for (int i = b; i < e; ++i) {
       float v[SpVec<E>::N];
-      SpVec<E>::get(sl.again(i), v);
+      SpVec<E>::get(sl.fetch(i), v);
 #pragma unroll
       for (int j = 0; j < SpVec<E>::N; ++j) mine += v[j] == m.value;
     }
@@ -438,17 +618,19 @@ struct SpRow {
       int left = m.nth - before;
       for (int i = b; i < e; ++i) {
         float v[SpVec<E>::N];
-        SpVec<E>::get(sl.again(i), v);
+        SpVec<E>::get(sl.fetch(i), v);
 #pragma unroll
         for (int j = 0; j < SpVec<E>::N; ++j)
           if (v[j] == m.value && left-- == 0) of(0).token = sl.id(i, j);
       }
     }
   }
-  __device__ void carry_out(const SpCmd& m) {
+  __device__ __noinline__ void carry_out(const SpCmd& m) {
+    SpShared& s = sp_shared();
+    if (m.op == SP_FIRST) first_pass(m);
     if (m.op == SP_PASS) pass(m);
     if (m.op == SP_HIST) {
-      for (int i = threadIdx.x; i < SP_BINS / 4; i += SP_NT) s.hist4[i] = make_uint4(0, 0, 0, 0);
+      s.hist4[threadIdx.x] = make_uint4(0, 0, 0, 0);
       __syncthreads();
       if (m.shift < 0) hist_by_value();
       else hist_by_key(m);
@@ -458,6 +640,7 @@ struct SpRow {
   }
   // CTA 0: s.cmd to every CTA, carried out by all; returns when all are done.
   __device__ void command() {
+    SpShared& s = sp_shared();
     __syncthreads();
     constexpr int W = sizeof(SpCmd) / 4;
     for (int i = threadIdx.x; i < W * (ranks - 1); i += SP_NT)
@@ -470,50 +653,85 @@ struct SpRow {
     cl.sync();
   }
   __device__ void obey() {
+    SpShared& s = sp_shared();
     for (;;) {
       cl.sync();
       const SpCmd m = s.cmd;
       if (m.op == SP_DONE) return;
       carry_out(m);
       cl.sync();
-      if (m.op == SP_GATHER) return;  // the last one: CTA 0 has all it needs
     }
   }
 
   // ---- CTA 0 ----------------------------------------------------------------------
   // The cluster's counts added up: hist4 becomes the counts before each bin, mass
-  // about the mass before each bin (n_b times the weight `centre` gives).
+  // about the mass before each bin: n_b times the weight at the bin's centre, or of a
+  // value in it where that is the only one, or where the type has few values (16 bits:
+  // a bin mostly holds one value many times).
   template <typename F>
-  __device__ int merge(F centre) {
-    uint4 n = make_uint4(0, 0, 0, 0);
-    for (int r = 0; r < ranks; ++r) {
-      const uint4 x = of(r).hist4[threadIdx.x];
-      n.x += x.x;
-      n.y += x.y;
-      n.z += x.z;
-      n.w += x.w;
+  __device__ __noinline__ int merge(F centre) {
+    SpShared& s = sp_shared();
+    int n[4] = {0, 0, 0, 0};
+    float x[4];
+#pragma unroll
+    for (int r = 0; r < SP_CLUSTER; ++r)
+      if (r < ranks) {
+        const uint4 c = of(r).hist4[threadIdx.x];
+        const float4 f = of(r).some4[threadIdx.x];
+        const uint32_t ci[4] = {c.x, c.y, c.z, c.w};
+        const float fi[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (ci[j]) x[j] = fi[j];
+          n[j] += (int)ci[j];
+        }
+      }
+    const int b = 4 * threadIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const float rate = (float)k.inv_t;
+    float m[4], mi = 0.f;
+    int ni = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      m[j] = !n[j] ? 0.f
+             : n[j] == 1 || sizeof(E) == 2 ? n[j] * __expf((x[j] - k.mx) * rate)
+                                           : n[j] * centre(b + j);
+      mi += m[j];
+      ni += n[j];
     }
-    const int b = 4 * threadIdx.x;
-    const float m0 = n.x ? n.x * centre(b) : 0.f, m1 = n.y ? n.y * centre(b + 1) : 0.f,
-                m2 = n.z ? n.z * centre(b + 2) : 0.f, m3 = n.w ? n.w * centre(b + 3) : 0.f;
-    int total;
-    float all;
-    const int at = sp_block_scan((int)(n.x + n.y + n.z + n.w), s.red_i, &total);
-    const float ma = sp_block_scan(m0 + m1 + m2 + m3, s.red_f, &all);
-    s.hist4[threadIdx.x] = make_uint4(at, at + n.x, at + n.x + n.y, at + n.x + n.y + n.z);
-    s.mass[b] = ma;
-    s.mass[b + 1] = ma + m0;
-    s.mass[b + 2] = ma + m0 + m1;
-    s.mass[b + 3] = ma + m0 + m1 + m2;
+    int at = sp_warp_scan(ni), total = 0;
+    float ma = sp_warp_scan(mi);
+    if (lane == 31) {
+      s.red_i[warp] = at;
+      s.red_f[warp] = ma;
+    }
+    __syncthreads();
+    at -= ni;
+    ma -= mi;
+    float all = 0.f;
+#pragma unroll
+    for (int w = 0; w < SP_NT / 32; ++w) {
+      const int c = s.red_i[w];
+      const float f = s.red_f[w];
+      if (w < warp) {
+        at += c;
+        ma += f;
+      }
+      total += c;
+      all += f;
+    }
+    s.hist4[threadIdx.x] = make_uint4(at, at + n[0], at + n[0] + n[1], at + n[0] + n[1] + n[2]);
+    *reinterpret_cast<float4*>(&s.mass[b]) = make_float4(ma, ma + m[0], ma + m[0] + m[1], ma + m[0] + m[1] + m[2]);
     if (threadIdx.x == SP_NT - 1) s.mass[SP_BINS] = all;
     __syncthreads();
     return total;
   }
   __device__ __forceinline__ int before(int b, int total) const {
+    SpShared& s = sp_shared();
     return b >= SP_BINS ? total : reinterpret_cast<const int*>(s.hist4)[b];
   }
   // The bin of the k-th value (1 <= k <= total).
-  __device__ int bin_of_count(int k, int total) {
+  __device__ __noinline__ int bin_of_count(int k, int total) {
+    SpShared& s = sp_shared();
     for (int b = 4 * threadIdx.x; b < 4 * (int)threadIdx.x + 4; ++b)
       if (before(b, total) < k && k <= before(b + 1, total)) s.got_i = b;
     __syncthreads();
@@ -522,7 +740,8 @@ struct SpRow {
     return r;
   }
   // About the bin where the mass passes m; the last filled bin where none does.
-  __device__ int bin_of_mass(float m, int total) {
+  __device__ __noinline__ int bin_of_mass(float m, int total) {
+    SpShared& s = sp_shared();
     if (threadIdx.x == 0) s.got_i = -1;
     __syncthreads();
     for (int b = 4 * threadIdx.x; b < 4 * (int)threadIdx.x + 4; ++b)
@@ -533,57 +752,93 @@ struct SpRow {
     __syncthreads();
     return r >= 0 ? r : bin_of_count(total, total);
   }
-  // The bins around b that one window's list holds: *a .. *z.
+  // A window around bin b: its neighbours too, in [low, high], while they are small
+  // (a guess is rarely off by more), the bin alone where it is not.
   __device__ void window_of(int b, int low, int high, int total, int* a, int* z) {
-    *a = *z = b;
-    for (int i = 0; i < 16; ++i) {
-      if (*a > low && before(*z + 1, total) - before(*a - 1, total) <= SP_CAP) --*a;
-      if (*z < high && before(*z + 2, total) - before(*a, total) <= SP_CAP) ++*z;
-    }
+    SpShared& s = sp_shared();
+    const int l1 = max(low, b - 1), l2 = max(low, b - 2), h1 = min(high, b + 1), h2 = min(high, b + 2);
+    const int up2 = before(l2, total), up1 = before(l1, total), down1 = before(h1 + 1, total),
+              down2 = before(h2 + 1, total);
+    const bool two = down2 - up2 <= SP_WIDEN, one = down1 - up1 <= SP_RANKED;
+    *a = two ? l2 : one ? l1 : b;
+    *z = two ? h2 : one ? h1 : b;
   }
   // The largest key whose value falls into bin b or a later one (one below the
   // least finite key where none does): bins are monotone in the value.
-  __device__ uint32_t top_of_bin(int b) const {
-    uint32_t lo = sp_key(-FLT_MAX) - 1, hi = sp_key(mx);
+  __device__ __noinline__ uint32_t top_of_bin(int b) const {
+    SpShared& s = sp_shared();
+    uint32_t lo = sp_key(-FLT_MAX) - 1, hi = sp_key(k.mx);
     if (b <= 0) return hi;
     if (b >= SP_BINS) return lo;
     while (lo < hi) {
       const uint32_t mid = lo + (hi - lo + 1) / 2;
-      if (bin(sp_value(mid)) >= b) lo = mid;
+      if (k.bin(sp_value(mid)) >= b) lo = mid;
       else hi = mid - 1;
     }
     return lo;
   }
-  // Sorted list -> this thread's four prefix sums and weights.
+  // Sorted list -> this thread's prefix sums and weights, entries i = PER t + j.
+  template <int PER>
   __device__ void prefixes(const unsigned long long* list, int n, double* w, double* sum) {
+    SpShared& s = sp_shared();
     double mine = 0.0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = 4 * threadIdx.x + j;
-      w[j] = i < n ? weight_any(sp_value((uint32_t)(list[i] >> 32))) : 0.0;
+    for (int j = 0; j < PER; ++j) {
+      const int i = PER * threadIdx.x + j;
+      w[j] = i < n ? k.weight_any(sp_value((uint32_t)(list[i] >> 32))) : 0.0;
       mine += w[j];
     }
     double all;
     double run = sp_block_scan(mine, s.red_d, &all);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum[j] = run += w[j];
+    for (int j = 0; j < PER; ++j) sum[j] = run += w[j];
   }
+  template <int PER>
   __device__ double sum_at(const double* sum, int i) {
-    if (i / 4 == (int)threadIdx.x) s.got_d = sum[i & 3];
+    SpShared& s = sp_shared();
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (PER * (int)threadIdx.x + j == i) s.got_d = sum[j];
     __syncthreads();
     const double r = s.got_d;
     __syncthreads();
     return r;
   }
+  // How many of the entries satisfy a condition.
+  template <int PER, typename F>
+  __device__ int count(F holds) {
+    SpShared& s = sp_shared();
+    if constexpr (PER == 1) return __syncthreads_count(holds(0));
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) n += holds(j);
+    return sp_block_sum(n, s.red_i);
+  }
+  // All of a row's decisions on the sorted list of its first n values.
+  template <int PER>
+  __device__ __noinline__ void decide(const SpArgs& a, int row, int n, int wanted, float top_p, float theta, float u) {
+    SpShared& s = sp_shared();
+    double w[PER], sum[PER];
+    prefixes<PER>(s.list, n, w, sum);
+    const int i0 = PER * (int)threadIdx.x;
+    int many = min(wanted, n);
+    if (top_p < 1.0f) {
+      const double want = (double)top_p * sum_at<PER>(sum, many - 1);
+      many = min(many, count<PER>([&](int j) { return i0 + j < many && sum[j] < want; }) + 1);
+    }
+    many = count<PER>([&](int j) {
+      return i0 + j < many && sp_value((uint32_t)(s.list[i0 + j] >> 32)) >= theta;
+    });
+    const double left = sum_at<PER>(sum, many - 1);
+    const int at = min(count<PER>([&](int j) { return i0 + j < many && sum[j] <= (double)u * left; }),
+                       many - 1);
+    if (threadIdx.x == 0) {
+      const unsigned long long e = s.list[at];
+      const double d = ((double)sp_value((uint32_t)(e >> 32)) - (double)k.mx) * k.inv_t;
+      sp_write(a, row, (int)(0xFFFFFFFFu - (uint32_t)e), (float)(d - log(left)), many, 0);
+    }
+  }
 };
-
-__device__ void sp_write(const SpArgs& a, int row, int token, float logprob, int kept,
-                         uint32_t flags) {
-  a.tokens[row] = token;
-  if (a.logprobs) a.logprobs[row] = logprob;
-  if (a.kept) a.kept[row] = kept;
-  if (a.flags) a.flags[row] = flags;
-}
 
 // A window of values in which a crossing is looked for.
 struct SpWindow {
@@ -595,12 +850,11 @@ struct SpWindow {
   bool gather;
 };
 
-template <typename E, bool RES>
+template <typename E>
 __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) {
-  extern __shared__ uint4 sp_slice[];
-  __shared__ SpShared s;
+  SpShared& s = sp_shared();
   constexpr int N = SpVec<E>::N;
-  SpRow<E, RES> R{s, {}, cg::this_cluster()};
+  SpRow<E> R{{}, cg::this_cluster()};
   R.rank = (int)R.cl.block_rank();
   R.ranks = (int)R.cl.num_blocks();
   const int row = blockIdx.x / R.ranks;
@@ -630,33 +884,18 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
     const int granules = (a.vocab + R.sl.skip + N - 1) / N;
     R.sl.g0 = min(granules, R.rank * a.per);
     R.sl.n = min(granules, (R.rank + 1) * a.per) - R.sl.g0;
-    R.sl.sm = sp_slice;
   }
-  if (t < 256) s.table[t] = exp2(t / 256.0);
-  for (int i = t; i < SP_BINS / 4; i += SP_NT) s.hist4[i] = make_uint4(0, 0, 0, 0);
+  s.hist4[t] = make_uint4(0, 0, 0, 0);
   if (t < SP_WINDOWS) s.n_list[t] = 0;
   float mx = -INFINITY, mn = INFINITY;
-  {
-    constexpr int U = 4;  // loads in flight per thread
-    for (int i0 = t; i0 < R.sl.n; i0 += U * SP_NT) {
-      uint4 g[U];
+  R.sl.template each<2>([&](const float* v, int) {
 #pragma unroll
-      for (int j = 0; j < U; ++j)
-        if (i0 + j * SP_NT < R.sl.n) g[j] = R.sl.fetch(i0 + j * SP_NT);
-#pragma unroll
-      for (int j = 0; j < U; ++j)
-        if (i0 + j * SP_NT < R.sl.n) {
-          if constexpr (RES) sp_slice[i0 + j * SP_NT] = g[j];
-          float v[N];
-          SpVec<E>::get(g[j], v);
-#pragma unroll
-          for (int e = 0; e < N; ++e) {
-            mx = sp_max_nan(mx, v[e]);
-            mn = fminf(mn, v[e] == -INFINITY ? INFINITY : v[e]);
-          }
-        }
+    for (int e = 0; e < N; ++e) {
+      mx = sp_max_nan(mx, v[e]);
+      mn = fminf(mn, v[e] == -INFINITY ? INFINITY : v[e]);
     }
-  }
+  });
+  const float own = mx;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     mx = sp_max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -688,7 +927,7 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
       sp_write(a, row, -1, __uint_as_float(0x7FC00000u), 0, NCB_FLAG_NONFINITE);
     return;
   }
-  R.mx = mx;
+  R.k.mx = mx;
   if (greedy) {
     SpCmd m{};
     m.op = SP_SELECT;
@@ -698,73 +937,94 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
     if (R.rank == 0 && t == 0) sp_write(a, row, s.token, 0.0f, 1, 0);
     return;
   }
-  R.inv_t = 1.0 / (double)T;
-  R.c = 256.0 / 0.69314718055994530942 * R.inv_t;
+  R.k.inv_t = 1.0 / (double)T;
+  R.k.c = R.k.inv_t / 0.69314718055994530942;
   // bins over the finite values, as far as they carry mass
   const double far = (double)mx - SP_REACH * (double)T;
-  R.zero = far > -(double)FLT_MAX ? (float)far : -FLT_MAX;
-  R.scale = (float)((SP_BINS - 1) / ((double)mx - fmax((double)mn, far)));
+  R.k.zero = far > -(double)FLT_MAX ? (float)far : -FLT_MAX;
+  R.k.scale = (float)fmin((SP_BINS - 1) / ((double)mx - fmax((double)mn, far)), (double)FLT_MAX);
 
-  // ---- counts ------------------------------------------------------------------------
-  R.hist_by_value();
-  R.cl.sync();
+  // ---- few values wanted: those above a bound ------------------------------------------
+  // The threads' maxima are so many different values of the row: the bin of the k-th
+  // largest of them, or an earlier one, holds the k-th value.
+  const bool bounded = k_asked > 0 && k_asked <= min(SP_BOUNDED, SP_NT * R.ranks / 2);
+  const bool few = bounded || (min_p > 0.0f && top_p >= 1.0f);
+  if (few) {
+    if (bounded && own > -INFINITY) atomicAdd(reinterpret_cast<int*>(s.hist4) + R.k.bin(own), 1);
+    R.cl.sync();
+  } else {
+    R.hist_by_value();
+    R.cl.sync();
+  }
   if (R.rank != 0) {
     R.obey();
     return;
   }
-  const float step = (float)(R.inv_t / (double)R.scale);  // nats per bin
-  auto centre = [&](int b) { return __expf(-((float)b + 0.5f) * step); };
-  const int total = R.merge(centre);
-  const int k = k_asked > 0 && k_asked < total ? k_asked : total;
   // the least value that min-p keeps: w >= m  <=>  x >= max + T ln m
-  float theta = -FLT_MAX;
-  if (min_p > 0.0f) {
-    const double edge = log((double)min_p), least = (double)mx + edge * (double)T;
-    theta = least > -(double)FLT_MAX ? (float)least : -FLT_MAX;
-    auto kept = [&](float v) { return ((double)v - (double)mx) * R.inv_t >= edge; };
-    while (theta < mx && !kept(theta)) theta = nextafterf(theta, INFINITY);
-    while (theta > -FLT_MAX && kept(nextafterf(theta, -INFINITY))) theta = nextafterf(theta, -INFINITY);
+  if (t == 0) {
+    float least = -FLT_MAX;
+    if (min_p > 0.0f) {
+      const double edge = log((double)min_p), at = (double)mx + edge * (double)T;
+      least = at > -(double)FLT_MAX ? (float)at : -FLT_MAX;
+      auto kept = [&](float v) { return ((double)v - (double)mx) * R.k.inv_t >= edge; };
+      while (least < mx && !kept(least)) least = nextafterf(least, INFINITY);
+      while (least > -FLT_MAX && kept(nextafterf(least, -INFINITY))) least = nextafterf(least, -INFINITY);
+    }
+    s.theta = least;
   }
-  const int bk = R.bin_of_count(k, total);
-  const int bm = R.bin(theta);
-  // the last bin that has to be known: all of K where its mass is asked for
-  const int deep = top_p < 1.0f ? bk : min(bk, bm);
-
-  if (R.before(deep + 1, total) <= SP_LIST) {
-    // ---- few: one list decides ---------------------------------------------------------
+  const float step = (float)(R.k.inv_t / (double)R.k.scale);  // nats per bin
+  auto centre = [&](int b) { return __expf(-((float)b + 0.5f) * step); };
+  if (few) {
+    int deep = SP_BINS - 1;  // the last bin that has to be known
+    if (bounded) {
+      const int maxima = R.merge(centre);
+      if (maxima >= k_asked) deep = R.bin_of_count(k_asked, maxima);
+    }
+    __syncthreads();
+    if (min_p > 0.0f && top_p >= 1.0f) deep = min(deep, R.k.bin(s.theta));
     if (t == 0) {
       s.cmd.op = SP_GATHER;
-      s.cmd.bin = deep;
+      s.cmd.below[0] = deep == SP_BINS - 1 ? INFINITY : (float)(deep + 1);
     }
     R.command();
     const int n = s.n_list[0];
-    sp_sort(s.list, n);
-    double w[4], sum[4];
-    R.prefixes(s.list, n, w, sum);
-    const int i0 = 4 * t;
-    int many = min(k, n);
-    if (top_p < 1.0f) {
-      const double want = (double)top_p * R.sum_at(sum, many - 1);
-      int less = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) less += i0 + j < many && sum[j] < want;
-      many = min(many, sp_block_sum(less, s.red_i) + 1);
+    if (n <= SP_FEW) {
+      if (t == 0) s.cmd.op = SP_DONE;
+      R.command();
+      sp_sort(s.list, n);
+      const int k = k_asked > 0 ? k_asked : n;  // (fewer finite values than k: all of them are here)
+      if (n <= SP_NT) R.template decide<1>(a, row, n, k, top_p, s.theta, u);
+      else R.template decide<SP_FEW / SP_NT>(a, row, n, k, top_p, s.theta, u);
+      return;
     }
-    int fit = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      fit += i0 + j < many && sp_value((uint32_t)(s.list[min(i0 + j, SP_LIST - 1)] >> 32)) >= theta;
-    many = sp_block_sum(fit, s.red_i);
-    const double left = R.sum_at(sum, many - 1);
-    int passed = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) passed += i0 + j < many && sum[j] <= (double)u * left;
-    const int at = min(sp_block_sum(passed, s.red_i), many - 1);
     if (t == 0) {
-      const unsigned long long e = s.list[at];
-      const double d = ((double)sp_value((uint32_t)(e >> 32)) - (double)mx) * R.inv_t;
-      sp_write(a, row, (int)(0xFFFFFFFFu - (uint32_t)e), (float)(d - log(left)), many, 0);
+      s.cmd.op = SP_HIST;
+      s.cmd.shift = -1;
     }
+    R.command();
+  }
+  const int total = R.merge(centre);
+  const int k = k_asked > 0 && k_asked < total ? k_asked : total;
+  const int bk = R.bin_of_count(k, total);
+  const float theta = s.theta;  // (written before merge's barriers)
+  const int bm = R.k.bin(theta);
+  // the last bin that has to be known: all of K where its mass is asked for
+  const int deep = top_p < 1.0f ? bk : min(bk, bm);
+
+  if (R.before(deep + 1, total) <= SP_FEW) {
+    // ---- few: one list decides ---------------------------------------------------------
+    if (t == 0) {
+      s.cmd.op = SP_GATHER;
+      s.cmd.below[0] = deep == SP_BINS - 1 ? INFINITY : (float)(deep + 1);
+      s.n_list[0] = 0;
+    }
+    R.command();
+    if (t == 0) s.cmd.op = SP_DONE;
+    R.command();
+    const int n = s.n_list[0];
+    sp_sort(s.list, n);
+    if (n <= SP_NT) R.template decide<1>(a, row, n, k, top_p, theta, u);
+    else R.template decide<SP_FEW / SP_NT>(a, row, n, k, top_p, theta, u);
     return;
   }
 
@@ -802,15 +1062,18 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
     R.merge(centre);
     by_value = true;
   };
-  // A window's keys from its bins; its values are listed where they fit.
+  // A window of bins: listed where it fits, and its keys, which only the general pass
+  // asks for.
   auto set_bins = [&](int w) {
+    win[w].by_key = false;
+    win[w].gather = R.before(win[w].z + 1, total) - R.before(win[w].a, total) <= SP_CAP;
+  };
+  auto set_keys = [&](int w) {
     if (t < 2) s.tops[t] = R.top_of_bin(t == 0 ? win[w].a : win[w].z + 1);
     __syncthreads();
     win[w].khi = s.tops[0];
     win[w].klo = s.tops[1] + 1;
     __syncthreads();
-    win[w].by_key = false;
-    win[w].gather = R.before(win[w].z + 1, total) - R.before(win[w].a, total) <= SP_CAP;
   };
   for (int w = 0; w < SP_WINDOWS; ++w)
     if (!found[w]) set_bins(w);
@@ -832,7 +1095,7 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
     const uint32_t half = shift ? 1u << (shift - 1) : 0u;
     const int n = R.merge([&](int b) {
       const uint32_t key = hi - min(((uint32_t)b << shift) + half, hi - lo);
-      return (float)R.weight_any(sp_value(key));
+      return (float)R.k.weight_any(sp_value(key));
     });
     int a1, z1;
     if (count) {
@@ -856,12 +1119,20 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
   // Each turn finds a crossing or leaves it fewer values (a neighbouring window, or
   // the part of one that holds it), so the loop ends; the limit is a guard.
   for (int turn = 0; !found[SP_D] && turn < SP_TURNS; ++turn) {
+    bool first = true;  // all windows are runs of bins: the first pass will do
+    for (int w = 0; w < SP_WINDOWS; ++w) first = first && (found[w] || !win[w].by_key);
+    if (!first)
+      for (int w = 0; w < SP_WINDOWS; ++w)
+        if (!found[w] && !win[w].by_key) set_keys(w);
+    if (first) need_bins();
     if (t == 0) {
-      s.cmd.op = SP_PASS;
+      s.cmd.op = first ? SP_FIRST : SP_PASS;
       s.cmd.theta = theta;
       for (int w = 0; w < SP_WINDOWS; ++w) {
         // a window that is not looked at any more: nothing in it, and above it every
         // value for K (whose mass is then the row's), none for the others
+        s.cmd.above[w] = found[w] ? (w == SP_K ? INFINITY : 0.0f) : (float)win[w].a;
+        s.cmd.below[w] = found[w] ? 0.0f : win[w].z == SP_BINS - 1 ? INFINITY : (float)(win[w].z + 1);
         s.cmd.klo[w] = found[w] ? 0xFFFFFFFFu : win[w].klo;
         s.cmd.khi[w] = found[w] ? (w == SP_K ? sp_key(-INFINITY) : sp_key(INFINITY)) : win[w].khi;
         s.cmd.gather[w] = !found[w] && win[w].gather;
@@ -877,6 +1148,22 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
         p.n[j] += s.part[r].n[j];
       }
     }
+    if (first)  // counts are known; what is in the windows comes with their lists
+      for (int w = 0; w < SP_WINDOWS; ++w) {
+        if (found[w]) continue;
+        p.n[w] = R.before(win[w].a, total);
+        p.n[SP_WINDOWS + 1 + w] = R.before(win[w].z + 1, total) - p.n[w];
+        if (!win[w].gather) {  // or is one value, or needs its mass from the other pass
+          uint32_t low = 0xFFFFFFFFu, high = 0;
+          for (int r = 0; r < R.ranks; ++r) {
+            low = min(low, s.k_low[r][w]);
+            high = max(high, s.k_high[r][w]);
+          }
+          win[w].klo = low;
+          win[w].khi = high;
+          p.mass[SP_WINDOWS + 1 + w] = low == high ? p.n_in(w) * R.k.weight_any(sp_value(low)) : -1.0;
+        }
+      }
     // K ends at the k-th value, counted: its window holds it.
     if (!by_k) {
       mass_k = p.above(SP_K);
@@ -885,14 +1172,14 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
       SpWindow& v = win[SP_K];
       if (v.gather) {
         sp_sort(s.list + SP_K * SP_CAP, p.n_in(SP_K));
-        double w[4], sum[4];
-        R.prefixes(s.list + SP_K * SP_CAP, p.n_in(SP_K), w, sum);
-        mass_k = p.above(SP_K) + R.sum_at(sum, idx - 1);
+        double w[1], sum[1];
+        R.template prefixes<1>(s.list + SP_K * SP_CAP, p.n_in(SP_K), w, sum);
+        mass_k = p.above(SP_K) + R.template sum_at<1>(sum, idx - 1);
         found[SP_K] = true;
       } else if (v.klo == v.khi) {
-        mass_k = p.above(SP_K) + idx * R.weight_any(sp_value(v.klo));
+        mass_k = p.above(SP_K) + idx * R.k.weight_any(sp_value(v.klo));
         found[SP_K] = true;
-      } else {
+      } else {  // (the least and greatest key, or the keys of its bins: k is between them)
         divide(SP_K, v.klo, v.khi, 0.0, p.n_above(SP_K), (double)k, true);
         continue;
       }
@@ -901,31 +1188,38 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
     // or of the equal values, 1 the window has moved.
     auto cross = [&](int w, double want, bool beyond, int* at, double* mass) -> int {
       SpWindow& v = win[w];
-      const double ab = p.above(w), in = p.in(w);
+      const double ab = p.above(w);
       auto past = [&](double x) { return beyond ? x > want : x >= want; };
-      const bool here = v.gather || v.klo == v.khi;
-      const bool up = past(ab) && p.n_above(w) > 0, down = !up && !past(ab + in);
-      if (!up && !down && here) {
-        if (v.gather) {
-          const unsigned long long* list = s.list + w * SP_CAP;
-          const int n = p.n_in(w);
-          double wt[4], sum[4];
-          sp_sort(s.list + w * SP_CAP, n);
-          R.prefixes(list, n, wt, sum);
-          int less = 0;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) less += 4 * t + j < n && !past(ab + sum[j]);
-          *at = min(sp_block_sum(less, s.red_i), n - 1);
-          *mass = ab + R.sum_at(sum, *at);
-        } else {
-          const double wt = R.weight_any(sp_value(v.klo));
-          double j = floor((want - ab) / wt);  // values passed before, give or take one
-          if (j > 0.0 && past(ab + j * wt)) j -= 1.0;
-          if (!past(ab + (j + 1.0) * wt)) j += 1.0;
-          *at = (int)fmin(fmax(j, 0.0), (double)(p.n_in(w) - 1));
-          *mass = ab + (*at + 1.0) * wt;
-        }
+      const bool up = past(ab) && p.n_above(w) > 0;
+      double in = p.in(w), wt = 0.0, sum[1] = {0.0};
+      const int n = p.n_in(w);
+      if (!up && v.gather) {  // the list says what is in the window
+        double each[1];
+        sp_sort(s.list + w * SP_CAP, n);
+        R.template prefixes<1>(s.list + w * SP_CAP, n, each, sum);
+        if (first) in = n ? R.template sum_at<1>(sum, n - 1) : 0.0;
+      }
+      const bool down = !up && in >= 0.0 && !past(ab + in);
+      if (!up && !down && v.gather) {
+        *at = min(R.template count<1>([&](int) { return t < n && !past(ab + sum[0]); }), n - 1);
+        *mass = ab + R.template sum_at<1>(sum, *at);
         return 0;
+      }
+      if (!up && !down && !v.gather && v.klo == v.khi) {  // equal values
+        wt = R.k.weight_any(sp_value(v.klo));
+        double j = floor((want - ab) / wt);  // values passed before, give or take one
+        if (j > 0.0 && past(ab + j * wt)) j -= 1.0;
+        if (!past(ab + (j + 1.0) * wt)) j += 1.0;
+        *at = (int)fmin(fmax(j, 0.0), (double)(n - 1));
+        *mass = ab + (*at + 1.0) * wt;
+        return 0;
+      }
+      if (first && !v.gather && in < 0.0 && !up) {  // too many different values: their mass first
+        v.by_key = true;
+        v.klo0 = sp_key(-FLT_MAX);
+        v.khi0 = v.khi;
+        v.above0 = ab;
+        return 1;
       }
       if (!v.by_key) {
         if (up && v.a > 0) {  // the bins just before
@@ -990,7 +1284,7 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
     if (!found[SP_D]) sp_write(a, row, -1, __uint_as_float(0x7FC00000u), 0, NCB_FLAG_TIES_OVERFLOW);
   }
   if (t == 0 && found[SP_D]) {
-    const double d = ((double)token_value - (double)mx) * R.inv_t;
+    const double d = ((double)token_value - (double)mx) * R.k.inv_t;
     sp_write(a, row, token, (float)(d - log(left)), many, 0);
   }
   R.command();
@@ -1000,25 +1294,25 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
 
 namespace {
 
-// The dynamic shared memory a CTA may hold its slice in, per kernel and device
-// (raised once; setting it twice is harmless).
-constexpr int SP_DEVICES = 64;
-constexpr int SP_MAX_SLICE = 184 * 1024;  // of 227 KiB, beside SpShared
+static_assert(sizeof(nvs::SpShared) <= 48 * 1024, "needs no larger limit");
 
-template <typename E, bool RES>
-int sp_launch(const nvs::SpArgs& a, int rows, int ranks, size_t smem, int device, cudaStream_t st) {
-  auto kernel = nvs::sample_min_p_kernel<E, RES>;
-  static std::atomic<bool> raised[SP_DEVICES];
-  if (RES && !raised[device].load(std::memory_order_acquire)) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SP_MAX_SLICE) !=
-        cudaSuccess)
-      return NCB_ERROR_LAUNCH_FAILED;
-    raised[device].store(true, std::memory_order_release);
-  }
+template <typename E>
+int sp_launch(nvs::SpArgs a, int rows, int num_sms, cudaStream_t st) {
+  // Granules of a row, counting a first one that starts before it.
+  const int n = 16 / (int)sizeof(E);
+  const int granules = (a.vocab + n - 1) / n + 1;
+  // as many CTAs to a row as fill the GPU twice over, while each has a granule for
+  // every thread
+  int ranks = 1;
+  while (ranks < nvs::SP_CLUSTER && (int64_t)rows * ranks * 2 <= 2 * num_sms &&
+         granules / ranks >= 2 * nvs::SP_NT)
+    ranks *= 2;
+  a.per = (granules + ranks - 1) / ranks;
+  if ((int64_t)rows * ranks > 0x7FFFFFFFLL) return NCB_ERROR_CAPACITY;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)rows * ranks);
   cfg.blockDim = dim3(nvs::SP_NT);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = sizeof(nvs::SpShared);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -1026,25 +1320,9 @@ int sp_launch(const nvs::SpArgs& a, int rows, int ranks, size_t smem, int device
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? NCB_OK : NCB_ERROR_LAUNCH_FAILED;
-}
-
-template <typename E>
-int sp_dispatch(nvs::SpArgs a, int rows, int device, cudaStream_t st) {
-  // Granules of a row, counting a first one that starts before it.
-  const int n = 16 / (int)sizeof(E);
-  const int granules = (a.vocab + n - 1) / n + 1;
-  int ranks = 1;
-  // as many CTAs as fill the GPU, while each has work for its threads; then as many
-  // as let two CTAs share an SM
-  while (ranks < nvs::SP_CLUSTER && (int64_t)rows * ranks * 2 <= 296 && granules / ranks >= 512)
-    ranks *= 2;
-  while (ranks < nvs::SP_CLUSTER && (int64_t)granules * 16 / ranks > 72 * 1024) ranks *= 2;
-  a.per = (granules + ranks - 1) / ranks;
-  const size_t smem = (size_t)a.per * 16;
-  if ((int64_t)rows * ranks > 0x7FFFFFFFLL) return NCB_ERROR_CAPACITY;
-  if (smem <= (size_t)SP_MAX_SLICE) return sp_launch<E, true>(a, rows, ranks, smem, device, st);
-  return sp_launch<E, false>(a, rows, ranks, 0, device, st);
+  return cudaLaunchKernelEx(&cfg, nvs::sample_min_p_kernel<E>, a) == cudaSuccess
+             ? NCB_OK
+             : NCB_ERROR_LAUNCH_FAILED;
 }
 
 }  // namespace
@@ -1067,8 +1345,9 @@ extern "C" NCB_API int ncb_sample_rows_min_p_device(
   if ((reinterpret_cast<uintptr_t>(d_logits) & low) || (words & 3u))
     return ncb_record_status(NCB_ERROR_INVALID_ARGUMENT);
   if (vocab > nvs::SP_MAX_VOCAB) return ncb_record_status(NCB_ERROR_CAPACITY);
-  int device = 0;
-  if (cudaGetDevice(&device) != cudaSuccess || device >= SP_DEVICES)
+  int device = 0, num_sms = 0;
+  if (cudaGetDevice(&device) != cudaSuccess ||
+      cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
     return ncb_record_status(NCB_ERROR_NO_DEVICE);
   nvs::SpArgs a{};
   a.logits = d_logits;
@@ -1085,8 +1364,8 @@ extern "C" NCB_API int ncb_sample_rows_min_p_device(
   a.flags = d_flags;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int status;
-  if (dtype == NCB_DTYPE_F32) status = sp_dispatch<float>(a, rows, device, st);
-  else if (dtype == NCB_DTYPE_F16) status = sp_dispatch<__half>(a, rows, device, st);
-  else status = sp_dispatch<__nv_bfloat16>(a, rows, device, st);
+  if (dtype == NCB_DTYPE_F32) status = sp_launch<float>(a, rows, num_sms, st);
+  else if (dtype == NCB_DTYPE_F16) status = sp_launch<__half>(a, rows, num_sms, st);
+  else status = sp_launch<__nv_bfloat16>(a, rows, num_sms, st);
   return ncb_record_status(status);
 }

@@ -229,8 +229,8 @@ struct SpSlice {
   // f(values, granule) for this thread's granules, FLIGHT loads at a time. The whole
   // granules are read without a branch (the loads would wait for one another); past
   // the end the last one is read again and dropped.
-  template <int FLIGHT, typename F>
-  __device__ __forceinline__ void each(F f) const {
+  template <int FLIGHT, int THREADS, typename F>
+  __device__ __forceinline__ void each_granule(F f) const {
     constexpr int N = SpVec<E>::N;
     const int lo = n > 0 && g0 * N < skip ? 1 : 0;
     const int hi = n > lo && (g0 + n) * N - skip > vocab ? n - 1 : n;
@@ -238,30 +238,40 @@ struct SpSlice {
     uint4 g[FLIGHT];
     auto load = [&](int i0) {
 #pragma unroll
-      for (int j = 0; j < FLIGHT; ++j) g[j] = __ldg(from + min(i0 + j * SP_NT, hi - 1));
+      for (int j = 0; j < FLIGHT; ++j) g[j] = __ldg(from + min(i0 + j * THREADS, hi - 1));
     };
     const int i0 = lo + threadIdx.x;
     if (lo < hi) load(i0);
 #pragma unroll 1
-    for (int i = i0; i < hi; i += FLIGHT * SP_NT) {
+    for (int i = i0; i < hi; i += FLIGHT * THREADS) {
       uint4 now[FLIGHT];
 #pragma unroll
       for (int j = 0; j < FLIGHT; ++j) now[j] = g[j];
-      load(i + FLIGHT * SP_NT);  // on its way while f works
+      load(i + FLIGHT * THREADS);  // on its way while f works
 #pragma unroll
       for (int j = 0; j < FLIGHT; ++j)
-        if (i + j * SP_NT < hi) {
-          float v[N];
-          SpVec<E>::get(now[j], v);
-          f(v, i + j * SP_NT);
-        }
+        if (i + j * THREADS < hi) f(now[j], i + j * THREADS);
     }
     const int edge = threadIdx.x == 0 && lo ? 0 : threadIdx.x == 32 && hi < n ? n - 1 : -1;
-    if (edge >= 0) {
-      float v[N];
-      SpVec<E>::get(fetch(edge), v);
-      f(v, edge);
-    }
+    if (edge >= 0) f(fetch(edge), edge);
+  }
+  template <int FLIGHT, typename F>
+  __device__ __forceinline__ void each(F f) const {
+    each_granule<FLIGHT, SP_NT>([&](const uint4& g, int i) {
+      float v[SpVec<E>::N];
+      SpVec<E>::get(g, v);
+      f(v, i);
+    });
+  }
+  // Of the row at x, the part of CTA `rank`: `per` granules.
+  __device__ __forceinline__ void set(const E* x, int vocab_, int rank, int per) {
+    constexpr int N = SpVec<E>::N;
+    skip = (int)((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(E));
+    base = reinterpret_cast<const char*>(x - skip);
+    vocab = vocab_;
+    const int granules = (vocab + skip + N - 1) / N;
+    g0 = min(granules, rank * per);
+    n = min(granules, (rank + 1) * per) - g0;
   }
   __device__ __forceinline__ int id(int i, int e) const {
     return (g0 + i) * SpVec<E>::N - skip + e;
@@ -368,6 +378,35 @@ __device__ void sp_write(const SpArgs& a, int row, int token, float logprob, int
   if (a.logprobs) a.logprobs[row] = logprob;
   if (a.kept) a.kept[row] = kept;
   if (a.flags) a.flags[row] = flags;
+}
+
+__device__ void sp_write_bad(const SpArgs& a, int row, uint32_t flag) {
+  sp_write(a, row, -1, __uint_as_float(0x7FC00000u), 0, flag);
+}
+
+struct SpOptions {
+  float T, top_p, min_p, u;
+  int top_k;
+  __device__ __forceinline__ bool read(const SpArgs& a, int row) {
+    T = a.temperature ? a.temperature[row] : 1.0f;
+    top_k = a.top_k ? a.top_k[row] : 0;
+    top_p = a.top_p ? a.top_p[row] : 1.0f;
+    min_p = a.min_p ? a.min_p[row] : 0.0f;
+    u = a.uniforms[row];
+    return T >= 0.0f && T <= FLT_MAX &&
+           (T == 0.0f || (top_p > 0.0f && min_p >= 0.0f && min_p <= 1.0f && u >= 0.0f && u < 1.0f));
+  }
+};
+
+// The least value that min-p keeps: w >= m  <=>  x >= max + T ln m.
+__device__ float sp_least_kept(float mx, float T, float min_p, double inv_t) {
+  if (!(min_p > 0.0f)) return -FLT_MAX;
+  const double edge = log((double)min_p), at = (double)mx + edge * (double)T;
+  float least = at > -(double)FLT_MAX ? (float)at : -FLT_MAX;
+  auto kept = [&](float v) { return ((double)v - (double)mx) * inv_t >= edge; };
+  while (least < mx && !kept(least)) least = nextafterf(least, INFINITY);
+  while (least > -FLT_MAX && kept(nextafterf(least, -INFINITY))) least = nextafterf(least, -INFINITY);
+  return least;
 }
 
 // What a value of the row means. The passes work on a copy of their own: behind a
@@ -844,6 +883,7 @@ struct SpRow {
 struct SpWindow {
   int a, z;             // its bins (by_key: unused)
   bool by_key;          // found by a histogram of keys inside [klo0, khi0]
+  bool weigh;           // a run of bins that does not fit: its own mass is needed too
   uint32_t klo, khi;    // its keys
   uint32_t klo0, khi0;  // by_key: keys between which the crossing is known to lie,
   double above0;        //   and the mass above them
@@ -861,30 +901,18 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
   const int t = threadIdx.x;
 
   // ---- options: the same for every CTA of the row -------------------------------
-  const float T = a.temperature ? a.temperature[row] : 1.0f;
-  const int k_asked = a.top_k ? a.top_k[row] : 0;
-  const float top_p = a.top_p ? a.top_p[row] : 1.0f;
-  const float min_p = a.min_p ? a.min_p[row] : 0.0f;
-  const float u = a.uniforms[row];
-  const bool greedy = T == 0.0f;
-  if (!(T >= 0.0f && T <= FLT_MAX) ||
-      (!greedy && !(top_p > 0.0f && min_p >= 0.0f && min_p <= 1.0f && u >= 0.0f && u < 1.0f))) {
-    if (R.rank == 0 && t == 0)
-      sp_write(a, row, -1, __uint_as_float(0x7FC00000u), 0, NCB_FLAG_BAD_OPTIONS);
+  SpOptions o;
+  if (!o.read(a, row)) {
+    if (R.rank == 0 && t == 0) sp_write_bad(a, row, NCB_FLAG_BAD_OPTIONS);
     return;
   }
+  const float T = o.T, top_p = o.top_p, min_p = o.min_p, u = o.u;
+  const int k_asked = o.top_k;
+  const bool greedy = T == 0.0f;
 
   R.cl.barrier_arrive();  // this CTA runs: the others may write into it
   // ---- load, maximum, least finite value ---------------------------------------------
-  {
-    const char* x = static_cast<const char*>(a.logits) + (int64_t)row * a.ld * (int64_t)sizeof(E);
-    R.sl.skip = (int)((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(E));
-    R.sl.base = x - R.sl.skip * (int)sizeof(E);
-    R.sl.vocab = a.vocab;
-    const int granules = (a.vocab + R.sl.skip + N - 1) / N;
-    R.sl.g0 = min(granules, R.rank * a.per);
-    R.sl.n = min(granules, (R.rank + 1) * a.per) - R.sl.g0;
-  }
+  R.sl.set(static_cast<const E*>(a.logits) + (int64_t)row * a.ld, a.vocab, R.rank, a.per);
   s.hist4[t] = make_uint4(0, 0, 0, 0);
   if (t < SP_WINDOWS) s.n_list[t] = 0;
   float mx = -INFINITY, mn = INFINITY;
@@ -923,8 +951,7 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
     mn = fminf(mn, s.mn[r]);
   }
   if (!(mx >= -FLT_MAX && mx <= FLT_MAX)) {
-    if (R.rank == 0 && t == 0)
-      sp_write(a, row, -1, __uint_as_float(0x7FC00000u), 0, NCB_FLAG_NONFINITE);
+    if (R.rank == 0 && t == 0) sp_write_bad(a, row, NCB_FLAG_NONFINITE);
     return;
   }
   R.k.mx = mx;
@@ -960,18 +987,7 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
     R.obey();
     return;
   }
-  // the least value that min-p keeps: w >= m  <=>  x >= max + T ln m
-  if (t == 0) {
-    float least = -FLT_MAX;
-    if (min_p > 0.0f) {
-      const double edge = log((double)min_p), at = (double)mx + edge * (double)T;
-      least = at > -(double)FLT_MAX ? (float)at : -FLT_MAX;
-      auto kept = [&](float v) { return ((double)v - (double)mx) * R.k.inv_t >= edge; };
-      while (least < mx && !kept(least)) least = nextafterf(least, INFINITY);
-      while (least > -FLT_MAX && kept(nextafterf(least, -INFINITY))) least = nextafterf(least, -INFINITY);
-    }
-    s.theta = least;
-  }
+  if (t == 0) s.theta = sp_least_kept(mx, T, min_p, R.k.inv_t);
   const float step = (float)(R.k.inv_t / (double)R.k.scale);  // nats per bin
   auto centre = [&](int b) { return __expf(-((float)b + 0.5f) * step); };
   if (few) {
@@ -1065,7 +1081,7 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
   // A window of bins: listed where it fits, and its keys, which only the general pass
   // asks for.
   auto set_bins = [&](int w) {
-    win[w].by_key = false;
+    win[w].by_key = win[w].weigh = false;
     win[w].gather = R.before(win[w].z + 1, total) - R.before(win[w].a, total) <= SP_CAP;
   };
   auto set_keys = [&](int w) {
@@ -1120,7 +1136,7 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
   // the part of one that holds it), so the loop ends; the limit is a guard.
   for (int turn = 0; !found[SP_D] && turn < SP_TURNS; ++turn) {
     bool first = true;  // all windows are runs of bins: the first pass will do
-    for (int w = 0; w < SP_WINDOWS; ++w) first = first && (found[w] || !win[w].by_key);
+    for (int w = 0; w < SP_WINDOWS; ++w) first = first && (found[w] || !(win[w].by_key || win[w].weigh));
     if (!first)
       for (int w = 0; w < SP_WINDOWS; ++w)
         if (!found[w] && !win[w].by_key) set_keys(w);
@@ -1215,10 +1231,7 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
         return 0;
       }
       if (first && !v.gather && in < 0.0 && !up) {  // too many different values: their mass first
-        v.by_key = true;
-        v.klo0 = sp_key(-FLT_MAX);
-        v.khi0 = v.khi;
-        v.above0 = ab;
+        v.weigh = true;
         return 1;
       }
       if (!v.by_key) {
@@ -1281,7 +1294,7 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
   }
   if (t == 0) {
     s.cmd.op = SP_DONE;
-    if (!found[SP_D]) sp_write(a, row, -1, __uint_as_float(0x7FC00000u), 0, NCB_FLAG_TIES_OVERFLOW);
+    if (!found[SP_D]) sp_write_bad(a, row, NCB_FLAG_TIES_OVERFLOW);
   }
   if (t == 0 && found[SP_D]) {
     const double d = ((double)token_value - (double)mx) * R.k.inv_t;
@@ -1290,29 +1303,416 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
   R.command();
 }
 
+// ---- rows of 16-bit values ----------------------------------------------------------------
+// A 16-bit type has 65536 values, so a row's counts per value say all there is to say
+// about it: masses are counts times weights, exact, and there is nothing to guess or
+// to sort. One pass counts (a 16-bit counter per value, 128 KiB of shared memory: a
+// CTA counts at most 65535 values of the row), one more finds the token's occurrence.
+//
+// Values are numbered from the greatest down ("places"). Of the merged counts CTA r
+// of a cluster owns the r-th part of the places, a thread SQ_CODES / ranks of them in a
+// row. A crossing is found in three steps, the CTA (by their totals), the thread (by a
+// scan), the place (by a warp).
+constexpr int SQ_NT = 1024;
+constexpr int SQ_CODES = 65536 / SQ_NT;  // places per thread of a CTA alone
+constexpr int SQ_SLICE = 65535;          // values that a CTA may count
+constexpr int SQ_TILES = SQ_SLICE / 8 / SQ_NT + 2;
+
+struct SqHit {     // where a crossing lies
+  int n;           // values kept up to and with it
+  int nth;         // which of the place's values it is
+  int place;
+  double mass;     // of the n values
+};
+struct SqShared {
+  int tot_n[SP_CLUSTER], first[SP_CLUSTER], bad[SP_CLUSTER], found[SP_CLUSTER], here[SP_CLUSTER];
+  double tot_m[SP_CLUSTER];
+  double kept_m[SP_CLUSTER];  // mass of what min-p keeps; found: how many
+  SqHit hit[SP_WINDOWS];
+  int in_warp[SQ_TILES][SQ_NT / 32];  // occurrences of the token's value
+  int red_i[SQ_NT / 32];
+  double red_d[SQ_NT / 32];
+  int at, last;
+  int before_n;
+  double before_m;
+};
+
+template <typename E>
+struct SqType;
+template <>
+struct SqType<__nv_bfloat16> {
+  static constexpr uint32_t INF = 0x7F80u;
+  static __device__ __forceinline__ float value(uint32_t b) { return __uint_as_float(b << 16); }
+};
+template <>
+struct SqType<__half> {
+  static constexpr uint32_t INF = 0x7C00u;
+  static __device__ __forceinline__ float value(uint32_t b) {
+    return __half2float(__ushort_as_half((unsigned short)b));
+  }
+};
+// The bits of the value at a place: +values from the greatest to +0, then -0 to the least.
+__device__ __forceinline__ uint32_t sq_bits(int place) {
+  return place < 32768 ? 32767u - place : (uint32_t)place;
+}
+
+template <typename E>
+struct SqRow {
+  cg::cluster_group cl;
+  int rank, ranks, pairs;  // pairs of places per thread
+  SpView k;
+  int n, before_n;         // this thread's values, and those before them in the CTA
+  double mass, before_m;   // their masses
+
+  static __device__ __forceinline__ uint32_t* counts() { return reinterpret_cast<uint32_t*>(sp_raw); }
+  // Counts of places 2 m and 2 m + 1, over the cluster.
+  __device__ __forceinline__ void pair(int m, int* c0, int* c1) const {
+    uint32_t* w = counts() + (m < 16384 ? 16383 - m : m);
+    int lo = 0, hi = 0;
+#pragma unroll
+    for (int r = 0; r < SP_CLUSTER; ++r)
+      if (r < ranks) {
+        const uint32_t x = ranks == 1 ? *w : *cl.map_shared_rank(w, r);
+        lo += x & 0xFFFFu;
+        hi += x >> 16;
+      }
+    *c0 = m < 16384 ? hi : lo;
+    *c1 = m < 16384 ? lo : hi;
+  }
+  __device__ __forceinline__ double weight(int place) const {
+    const float v = SqType<E>::value(sq_bits(place));
+    return v >= k.zero ? k.weight(v) : 0.0;
+  }
+  __device__ __forceinline__ SqShared& of(SqShared& s, int r) const {
+    return *cl.map_shared_rank(&s, r);
+  }
+
+  // The first value, in the order of the row, that `past` holds for: past(number of
+  // values up to it, their mass). Every thread of the cluster calls it; the result is in
+  // every CTA's hit[w] after the next cluster barrier.
+  template <typename F>
+  __device__ void cross(SqShared& s, int w, F past) {
+    int owner = -1, base_count = 0, last = 0, last_base = 0;
+    double base_mass = 0.0, last_mass = 0.0;
+    for (int r = 0; r < ranks && owner < 0; ++r) {
+      if (s.tot_n[r]) last = r, last_base = base_count, last_mass = base_mass;
+      if (s.tot_n[r] && past(base_count + s.tot_n[r], base_mass + s.tot_m[r])) {
+        owner = r;
+        break;
+      }
+      base_count += s.tot_n[r];
+      base_mass += s.tot_m[r];
+    }
+    if (owner < 0) owner = last, base_count = last_base, base_mass = last_mass;
+    if (owner != rank) return;
+    if (threadIdx.x == 0) s.at = SQ_NT, s.last = 0;
+    __syncthreads();
+    if (n) {
+      if (past(base_count + before_n + n, base_mass + (before_m + mass))) atomicMin(&s.at, (int)threadIdx.x);
+      atomicMax(&s.last, (int)threadIdx.x);
+    }
+    __syncthreads();
+    const int t = s.at < SQ_NT ? s.at : s.last;
+    if (t == (int)threadIdx.x) {
+      s.before_n = base_count + before_n;
+      s.before_m = base_mass + before_m;
+    }
+    __syncthreads();
+    if (threadIdx.x >= 32) return;
+    // the thread's places, a pair per lane
+    const int lane = threadIdx.x;
+    int c0 = 0, c1 = 0;
+    double w0 = 0.0, w1 = 0.0;
+    const int m = (rank * SQ_NT + t) * pairs + lane;
+    if (lane < pairs) {
+      pair(m, &c0, &c1);
+      if (c0) w0 = weight(2 * m);
+      if (c1) w1 = weight(2 * m + 1);
+    }
+    const double m0 = c0 * w0, m1 = c1 * w1;
+    const int en = s.before_n + sp_warp_scan(c0 + c1);
+    const double em = s.before_m + sp_warp_scan(m0 + m1);
+    const uint32_t yes = __ballot_sync(0xffffffffu, (c0 | c1) && past(en, em)),
+                   any = __ballot_sync(0xffffffffu, (c0 | c1) != 0);
+    const int l = yes ? __ffs(yes) - 1 : 31 - __clz(any);
+    if (lane != l) return;
+    const int b0 = en - c0 - c1;
+    const double a0 = em - (m0 + m1);
+    const bool second = !c0 || (c1 && !past(b0 + c0, a0 + m0));
+    const int bn = second ? b0 + c0 : b0, c = second ? c1 : c0;
+    const double bm = second ? a0 + m0 : a0, wt = second ? w1 : w0;
+    // values of the place before the crossing: the least j with past(bn + j + 1, ...)
+    int lo = 0, hi = c - 1;
+    while (lo < hi) {
+      const int j = (lo + hi) / 2;
+      if (past(bn + j + 1, bm + (j + 1.0) * wt)) hi = j;
+      else lo = j + 1;
+    }
+    const SqHit h{bn + lo + 1, lo, 2 * m + (second ? 1 : 0), bm + (lo + 1.0) * wt};
+    for (int r = 0; r < ranks; ++r) of(s, r).hit[w] = h;
+  }
+};
+
+template <typename E>
+__global__ void __launch_bounds__(SQ_NT, 1) sample_min_p16_kernel(const SpArgs a) {
+  __shared__ SqShared s;
+  SqRow<E> R{cg::this_cluster()};
+  R.rank = (int)R.cl.block_rank();
+  R.ranks = (int)R.cl.num_blocks();
+  R.pairs = SQ_CODES / 2 / R.ranks;
+  const int row = blockIdx.x / R.ranks, t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  SpOptions o;
+  if (!o.read(a, row)) {
+    if (R.rank == 0 && t == 0) sp_write_bad(a, row, NCB_FLAG_BAD_OPTIONS);
+    return;
+  }
+  const bool greedy = o.T == 0.0f;
+  SpSlice<E> sl;
+  sl.set(static_cast<const E*>(a.logits) + (int64_t)row * a.ld, a.vocab, R.rank, a.per);
+
+  // ---- counts --------------------------------------------------------------------------
+  for (int i = t; i < 8192; i += SQ_NT) sp_raw[i] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  {
+    uint32_t* counts = R.counts();
+    constexpr uint32_t none = 0x8000u | SqType<E>::INF;  // -inf
+    sl.template each_granule<4, SQ_NT>([&](const uint4& g, int) {
+      const uint32_t w[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t lo = w[j] & 0xFFFFu, hi = w[j] >> 16;
+        if (lo != none) atomicAdd(&counts[lo >> 1], 1u << ((lo & 1) * 16));
+        if (hi != none) atomicAdd(&counts[hi >> 1], 1u << ((hi & 1) * 16));
+      }
+    });
+  }
+  R.cl.sync();
+
+  // ---- this thread's places: counts, then masses -----------------------------------------------
+  // Neighbouring lanes start at different words, so that they read different banks.
+  const int turn = lane * R.pairs / 32, m0 = (R.rank * SQ_NT + t) * R.pairs;
+  int first = 65536, bad = 0;
+  uint32_t filled = 0;  // pairs with a value
+  R.n = 0;
+  for (int i = 0; i < R.pairs; ++i) {
+    const int j = (i + turn) & (R.pairs - 1), m = m0 + j;
+    int c0, c1;
+    R.pair(m, &c0, &c1);
+    if (c0 | c1) {
+      R.n += c0 + c1;
+      filled |= 1u << j;
+      first = min(first, c0 ? 2 * m : 2 * m + 1);
+      const uint32_t b0 = sq_bits(2 * m), b1 = sq_bits(2 * m + 1);
+      bad |= (c0 && (b0 & 0x7FFFu) >= SqType<E>::INF) || (c1 && (b1 & 0x7FFFu) >= SqType<E>::INF);
+    }
+  }
+  {
+    const int wn = __reduce_add_sync(0xffffffffu, R.n), wf = __reduce_min_sync(0xffffffffu, first);
+    if (lane == 0) s.red_i[warp] = wn, s.in_warp[0][warp] = wf;
+    bad = __syncthreads_or(bad);
+    if (t < 32) {
+      const int cn = __reduce_add_sync(0xffffffffu, s.red_i[t]),
+                cf = __reduce_min_sync(0xffffffffu, s.in_warp[0][t]);
+      if (t < R.ranks) {
+        SqShared& to = R.of(s, t);
+        to.tot_n[R.rank] = cn;
+        to.first[R.rank] = cf;
+        to.bad[R.rank] = bad;
+      }
+    }
+    R.cl.sync();
+  }
+  int total = 0, top = 65536;
+  for (int r = 0; r < R.ranks; ++r) {
+    total += s.tot_n[r];
+    top = min(top, s.first[r]);
+    bad |= s.bad[r];
+  }
+  if (bad || total == 0) {
+    if (R.rank == 0 && t == 0) sp_write_bad(a, row, NCB_FLAG_NONFINITE);
+    return;
+  }
+  const float mx = SqType<E>::value(sq_bits(top));
+  SqHit draw{1, 0, top, 1.0};
+  int many = 1;
+  double left = 1.0;
+  R.k.mx = mx;
+  if (!greedy) {
+    R.k.inv_t = 1.0 / (double)o.T;
+    R.k.c = R.k.inv_t / 0.69314718055994530942;
+    const double far = (double)mx - SP_REACH * (double)o.T;
+    R.k.zero = far > -(double)FLT_MAX ? (float)far : -FLT_MAX;
+    R.mass = 0.0;
+    for (int i = 0; i < R.pairs; ++i) {
+      const int j = (i + turn) & (R.pairs - 1), m = m0 + j;
+      if (!(filled >> j & 1)) continue;
+      int c0, c1;
+      R.pair(m, &c0, &c1);
+      R.mass += c0 * R.weight(2 * m) + c1 * R.weight(2 * m + 1);
+    }
+    // prefixes over the CTA's threads
+    const int in = sp_warp_scan(R.n);
+    const double im = sp_warp_scan(R.mass);
+    if (lane == 31) s.red_i[warp] = in, s.red_d[warp] = im;
+    __syncthreads();
+    if (t < 32) {
+      const int wn = sp_warp_scan(s.red_i[t]);
+      const double wm = sp_warp_scan(s.red_d[t]);
+      if (t == 31)
+        for (int r = 0; r < R.ranks; ++r) R.of(s, r).tot_m[R.rank] = wm;
+      s.red_i[t] = wn - s.red_i[t];
+      s.red_d[t] = wm - s.red_d[t];
+    }
+    __syncthreads();
+    R.before_n = s.red_i[warp] + in - R.n;
+    R.before_m = s.red_d[warp] + (im - R.mass);
+    R.cl.sync();
+
+    // ---- K, and what min-p keeps ---------------------------------------------------------------
+    const int kk = o.top_k > 0 && o.top_k < total ? o.top_k : total;
+    double mass = 0.0;
+    for (int r = 0; r < R.ranks; ++r) mass += s.tot_m[r];
+    many = kk;
+    if (kk < total) R.cross(s, SP_K, [&](int n, double) { return n >= kk; });
+    if (o.min_p > 0.0f) {
+      __syncthreads();
+      if (t == 0) s.before_m = (double)sp_least_kept(mx, o.T, o.min_p, R.k.inv_t);
+      __syncthreads();
+      const float least = (float)s.before_m;
+      __syncthreads();
+      // the CTA that owns the last place at or above it adds up: places before the
+      // thread's, and the thread's own
+      int pn = 0;
+      double pm = 0.0;
+      for (int i = 0; i < R.pairs; ++i) {
+        if (!(filled >> i & 1)) continue;
+        int c0, c1;
+        R.pair(m0 + i, &c0, &c1);
+        if (c0 && SqType<E>::value(sq_bits(2 * (m0 + i))) >= least) pn += c0, pm += c0 * R.weight(2 * (m0 + i));
+        if (c1 && SqType<E>::value(sq_bits(2 * (m0 + i) + 1)) >= least) pn += c1, pm += c1 * R.weight(2 * (m0 + i) + 1);
+      }
+      pn = __reduce_add_sync(0xffffffffu, pn);
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) pm += __shfl_xor_sync(0xffffffffu, pm, x);
+      if (lane == 0) s.red_i[warp] = pn, s.red_d[warp] = pm;
+      __syncthreads();
+      if (t < 32) {
+        pn = __reduce_add_sync(0xffffffffu, s.red_i[t]);
+        pm = s.red_d[t];
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) pm += __shfl_xor_sync(0xffffffffu, pm, x);
+        if (t < R.ranks) {
+          R.of(s, t).found[R.rank] = pn;
+          R.of(s, t).kept_m[R.rank] = pm;
+        }
+      }
+    }
+    if (kk < total || o.min_p > 0.0f) R.cl.sync();
+    if (kk < total) mass = s.hit[SP_K].mass;
+    // ---- P ------------------------------------------------------------------------------------------
+    left = mass;
+    if (o.top_p < 1.0f) {
+      const double want = (double)o.top_p * mass;
+      R.cross(s, SP_P, [&](int, double x) { return x >= want; });
+      R.cl.sync();
+      if (s.hit[SP_P].n < many) {
+        many = s.hit[SP_P].n;
+        left = s.hit[SP_P].mass;
+      }
+    }
+    if (o.min_p > 0.0f) {
+      int pn = 0;
+      double pm = 0.0;
+      for (int r = 0; r < R.ranks; ++r) {
+        pn += s.found[r];
+        pm += s.kept_m[r];
+      }
+      if (pn < many) many = pn, left = pm;
+    }
+    // ---- the draw -------------------------------------------------------------------------------------
+    const double want = (double)o.u * left;
+    R.cross(s, SP_D, [&](int n, double x) { return x > want || n >= many; });
+    R.cl.sync();
+    draw = s.hit[SP_D];
+  }
+
+  // ---- the token: the nth value at the place, by id --------------------------------------------------
+  const float value = SqType<E>::value(sq_bits(draw.place));
+  int nth = draw.nth;
+  if (draw.place == 32768) {  // -0: as good as +0, whose values come before
+    int c0, plus;
+    R.pair(16383, &c0, &plus);
+    nth += plus;
+  }
+  const uint32_t want = sq_bits(draw.place), also = value == 0.0f ? want ^ 0x8000u : want;
+  auto matches = [&](const uint4& g) {  // bit e: value e of the granule is it
+    const uint32_t w[4] = {g.x, g.y, g.z, g.w};
+    uint32_t yes = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t lo = w[j] & 0xFFFFu, hi = w[j] >> 16;
+      yes |= (uint32_t)(lo == want || lo == also) << (2 * j) |
+             (uint32_t)(hi == want || hi == also) << (2 * j + 1);
+    }
+    return yes;
+  };
+  // tile i of the slice is SQ_NT granules, a warp's part of it 32
+  for (int i = warp; i < SQ_TILES; i += SQ_NT / 32) s.in_warp[i][lane] = 0;
+  __syncthreads();
+  sl.template each_granule<4, SQ_NT>([&](const uint4& g, int i) {
+    const uint32_t yes = matches(g);
+    if (yes) atomicAdd(&s.in_warp[i / SQ_NT][i % SQ_NT / 32], __popc(yes));
+  });
+  __syncthreads();
+  int mine = 0;  // thread i < SQ_TILES * 32: part i
+  if (t < SQ_TILES * 32) mine = s.in_warp[t / 32][t % 32];
+  const int inc = sp_warp_scan(mine);
+  if (lane == 31) s.red_i[warp] = inc;
+  __syncthreads();
+  int before = inc - mine, here = 0;
+  for (int w = 0; w < SQ_NT / 32; ++w) {
+    if (w < warp) before += s.red_i[w];
+    here += s.red_i[w];
+  }
+  if (R.ranks > 1) {
+    if (t < R.ranks) R.of(s, t).here[R.rank] = here;
+    R.cl.sync();
+    for (int r = 0; r < R.rank; ++r) before += s.here[r];
+  }
+  if (t == 0) s.at = -1;
+  __syncthreads();
+  if (mine && nth >= before && nth < before + mine) {
+    s.at = t;
+    s.last = nth - before;
+  }
+  __syncthreads();
+  if (s.at < 0 || t >= 32) return;
+  const int part = s.at * 32 + lane;  // this lane's granule
+  const uint32_t yes = part < sl.n ? matches(sl.fetch(part)) : 0;
+  const int upto = sp_warp_scan(__popc(yes)), skip = s.last - (upto - __popc(yes));
+  if (skip >= 0 && skip < __popc(yes)) {
+    uint32_t b = yes;
+    for (int i = 0; i < skip; ++i) b &= b - 1;
+    const double d = greedy ? 0.0 : ((double)value - (double)mx) * R.k.inv_t;
+    sp_write(a, row, sl.id(part, __ffs(b) - 1), (float)(d - log(left)), many, 0);
+  }
+}
+
 }  // namespace nvs
 
 namespace {
 
 static_assert(sizeof(nvs::SpShared) <= 48 * 1024, "needs no larger limit");
+constexpr int SP_DEVICES = 64;
 
-template <typename E>
-int sp_launch(nvs::SpArgs a, int rows, int num_sms, cudaStream_t st) {
-  // Granules of a row, counting a first one that starts before it.
-  const int n = 16 / (int)sizeof(E);
-  const int granules = (a.vocab + n - 1) / n + 1;
-  // as many CTAs to a row as fill the GPU twice over, while each has a granule for
-  // every thread
-  int ranks = 1;
-  while (ranks < nvs::SP_CLUSTER && (int64_t)rows * ranks * 2 <= 2 * num_sms &&
-         granules / ranks >= 2 * nvs::SP_NT)
-    ranks *= 2;
+int sp_start(void (*kernel)(nvs::SpArgs), nvs::SpArgs a, int rows, int granules, int ranks,
+             int threads, size_t smem, cudaStream_t st) {
   a.per = (granules + ranks - 1) / ranks;
   if ((int64_t)rows * ranks > 0x7FFFFFFFLL) return NCB_ERROR_CAPACITY;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)rows * ranks);
-  cfg.blockDim = dim3(nvs::SP_NT);
-  cfg.dynamicSmemBytes = sizeof(nvs::SpShared);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -1320,9 +1720,41 @@ int sp_launch(nvs::SpArgs a, int rows, int num_sms, cudaStream_t st) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, nvs::sample_min_p_kernel<E>, a) == cudaSuccess
-             ? NCB_OK
-             : NCB_ERROR_LAUNCH_FAILED;
+  return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? NCB_OK : NCB_ERROR_LAUNCH_FAILED;
+}
+
+template <typename E>
+int sp_launch(const nvs::SpArgs& a, int rows, int device, int num_sms, cudaStream_t st) {
+  // Granules of a row, counting a first one that starts before it.
+  const int n = 16 / (int)sizeof(E);
+  const int granules = (a.vocab + n - 1) / n + 1;
+  if constexpr (sizeof(E) == 2) {
+    // as many CTAs to a row as its values need, then as fill the GPU, one per SM
+    int ranks = 1;
+    while (ranks < nvs::SP_CLUSTER &&
+           ((granules + ranks - 1) / ranks * n > nvs::SQ_SLICE ||
+            ((int64_t)rows * ranks * 2 <= num_sms && granules / ranks >= 2 * nvs::SQ_NT)))
+      ranks *= 2;
+    if ((granules + ranks - 1) / ranks * n <= nvs::SQ_SLICE) {
+      constexpr int smem = 65536 * 2;
+      static std::atomic<bool> raised[SP_DEVICES];  // per device; raising it twice is harmless
+      if (device >= SP_DEVICES || !raised[device].load(std::memory_order_acquire)) {
+        if (cudaFuncSetAttribute(nvs::sample_min_p16_kernel<E>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+          return NCB_ERROR_LAUNCH_FAILED;
+        if (device < SP_DEVICES) raised[device].store(true, std::memory_order_release);
+      }
+      return sp_start(nvs::sample_min_p16_kernel<E>, a, rows, granules, ranks, nvs::SQ_NT, smem, st);
+    }
+  }
+  // as many CTAs to a row as fill the GPU twice over, while each has two granules for
+  // every thread
+  int ranks = 1;
+  while (ranks < nvs::SP_CLUSTER && (int64_t)rows * ranks * 2 <= 2 * num_sms &&
+         granules / ranks >= 2 * nvs::SP_NT)
+    ranks *= 2;
+  return sp_start(nvs::sample_min_p_kernel<E>, a, rows, granules, ranks, nvs::SP_NT,
+                  sizeof(nvs::SpShared), st);
 }
 
 }  // namespace
@@ -1364,8 +1796,8 @@ extern "C" NCB_API int ncb_sample_rows_min_p_device(
   a.flags = d_flags;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int status;
-  if (dtype == NCB_DTYPE_F32) status = sp_launch<float>(a, rows, num_sms, st);
-  else if (dtype == NCB_DTYPE_F16) status = sp_launch<__half>(a, rows, num_sms, st);
-  else status = sp_launch<__nv_bfloat16>(a, rows, num_sms, st);
+  if (dtype == NCB_DTYPE_F32) status = sp_launch<float>(a, rows, device, num_sms, st);
+  else if (dtype == NCB_DTYPE_F16) status = sp_launch<__half>(a, rows, device, num_sms, st);
+  else status = sp_launch<__nv_bfloat16>(a, rows, device, num_sms, st);
   return ncb_record_status(status);
 }

@@ -1310,12 +1310,13 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
 // CTA counts at most 65535 values of the row), one more finds the token's occurrence.
 //
 // Values are numbered from the greatest down ("places"). Of the merged counts CTA r
-// of a cluster owns the r-th part of the places, a thread SQ_CODES / ranks of them in a
-// row. A crossing is found in three steps, the CTA (by their totals), the thread (by a
-// scan), the place (by a warp).
+// of a cluster owns the r-th part of the places. It writes those that occur down as a
+// list of (place, count), which shares the weights out evenly among its threads (the
+// places that occur lie close together). A crossing is found by CTA (their totals),
+// then by thread (a scan), then by entry.
 constexpr int SQ_NT = 1024;
-constexpr int SQ_CODES = 65536 / SQ_NT;  // places per thread of a CTA alone
-constexpr int SQ_SLICE = 65535;          // values that a CTA may count
+constexpr int SQ_SLICE = 65535;  // values that a CTA may count
+constexpr int SQ_ALONE = 32768;  // and that a CTA alone may have: its list takes the counters' place
 constexpr int SQ_TILES = SQ_SLICE / 8 / SQ_NT + 2;
 
 struct SqHit {     // where a crossing lies
@@ -1325,16 +1326,14 @@ struct SqHit {     // where a crossing lies
   double mass;     // of the n values
 };
 struct SqShared {
-  int tot_n[SP_CLUSTER], first[SP_CLUSTER], bad[SP_CLUSTER], found[SP_CLUSTER], here[SP_CLUSTER];
-  double tot_m[SP_CLUSTER];
-  double kept_m[SP_CLUSTER];  // mass of what min-p keeps; found: how many
+  int tot_n[SP_CLUSTER], first[SP_CLUSTER], bad[SP_CLUSTER], kept_n[SP_CLUSTER], here[SP_CLUSTER];
+  double tot_m[SP_CLUSTER], kept_m[SP_CLUSTER];  // kept: what min-p keeps
   SqHit hit[SP_WINDOWS];
   int in_warp[SQ_TILES][SQ_NT / 32];  // occurrences of the token's value
-  int red_i[SQ_NT / 32];
-  double red_d[SQ_NT / 32];
+  int red_i[SQ_NT / 32], red_j[SQ_NT / 32];
+  double red_d[SQ_NT / 32], red_e[SQ_NT / 32];
+  float theta;
   int at, last;
-  int before_n;
-  double before_m;
 };
 
 template <typename E>
@@ -1356,29 +1355,23 @@ __device__ __forceinline__ uint32_t sq_bits(int place) {
   return place < 32768 ? 32767u - place : (uint32_t)place;
 }
 
-template <typename E>
+template <typename E, int RANKS>
 struct SqRow {
+  static constexpr int PLACES = 65536 / RANKS;      // of a CTA
+  static constexpr int PAIRS = PLACES / SQ_NT / 2;  // of a thread
   cg::cluster_group cl;
-  int rank, ranks, pairs;  // pairs of places per thread
+  int rank;
   SpView k;
+  int entries, per;        // of the CTA's list, of a thread
   int n, before_n;         // this thread's values, and those before them in the CTA
   double mass, before_m;   // their masses
 
+  // The counters, and then the list: place within the CTA's in the low bits, the count
+  // above it (the counts of RANKS slices need as many bits more as the places need
+  // fewer).
   static __device__ __forceinline__ uint32_t* counts() { return reinterpret_cast<uint32_t*>(sp_raw); }
-  // Counts of places 2 m and 2 m + 1, over the cluster.
-  __device__ __forceinline__ void pair(int m, int* c0, int* c1) const {
-    uint32_t* w = counts() + (m < 16384 ? 16383 - m : m);
-    int lo = 0, hi = 0;
-#pragma unroll
-    for (int r = 0; r < SP_CLUSTER; ++r)
-      if (r < ranks) {
-        const uint32_t x = ranks == 1 ? *w : *cl.map_shared_rank(w, r);
-        lo += x & 0xFFFFu;
-        hi += x >> 16;
-      }
-    *c0 = m < 16384 ? hi : lo;
-    *c1 = m < 16384 ? lo : hi;
-  }
+  __device__ __forceinline__ int place_of(uint32_t e) const { return rank * PLACES + (int)(e & (PLACES - 1)); }
+  static __device__ __forceinline__ int count_of(uint32_t e) { return (int)(e / PLACES); }
   __device__ __forceinline__ double weight(int place) const {
     const float v = SqType<E>::value(sq_bits(place));
     return v >= k.zero ? k.weight(v) : 0.0;
@@ -1392,75 +1385,61 @@ struct SqRow {
   // every CTA's hit[w] after the next cluster barrier.
   template <typename F>
   __device__ void cross(SqShared& s, int w, F past) {
-    int owner = -1, base_count = 0, last = 0, last_base = 0;
-    double base_mass = 0.0, last_mass = 0.0;
-    for (int r = 0; r < ranks && owner < 0; ++r) {
-      if (s.tot_n[r]) last = r, last_base = base_count, last_mass = base_mass;
-      if (s.tot_n[r] && past(base_count + s.tot_n[r], base_mass + s.tot_m[r])) {
+    int owner = -1, base_n = 0, last = 0, last_n = 0;
+    double base_m = 0.0, last_m = 0.0;
+#pragma unroll
+    for (int r = 0; r < RANKS; ++r) {
+      if (owner >= 0) continue;
+      if (s.tot_n[r]) last = r, last_n = base_n, last_m = base_m;
+      if (s.tot_n[r] && past(base_n + s.tot_n[r], base_m + s.tot_m[r])) {
         owner = r;
-        break;
+      } else {
+        base_n += s.tot_n[r];
+        base_m += s.tot_m[r];
       }
-      base_count += s.tot_n[r];
-      base_mass += s.tot_m[r];
     }
-    if (owner < 0) owner = last, base_count = last_base, base_mass = last_mass;
+    if (owner < 0) owner = last, base_n = last_n, base_m = last_m;
     if (owner != rank) return;
     if (threadIdx.x == 0) s.at = SQ_NT, s.last = 0;
     __syncthreads();
     if (n) {
-      if (past(base_count + before_n + n, base_mass + (before_m + mass))) atomicMin(&s.at, (int)threadIdx.x);
+      if (past(base_n + before_n + n, base_m + (before_m + mass))) atomicMin(&s.at, (int)threadIdx.x);
       atomicMax(&s.last, (int)threadIdx.x);
     }
     __syncthreads();
-    const int t = s.at < SQ_NT ? s.at : s.last;
-    if (t == (int)threadIdx.x) {
-      s.before_n = base_count + before_n;
-      s.before_m = base_mass + before_m;
+    if ((int)threadIdx.x != (s.at < SQ_NT ? s.at : s.last)) return;
+    int bn = base_n + before_n, c = 0, place = 0;
+    double bm = base_m + before_m, wt = 0.0;
+    const int i0 = threadIdx.x * per, i1 = min(entries, i0 + per);
+    for (int i = i0; i < i1; ++i) {
+      const uint32_t e = counts()[i];
+      place = place_of(e);
+      c = count_of(e);
+      wt = weight(place);
+      if (i == i1 - 1 || past(bn + c, bm + c * wt)) break;
+      bn += c;
+      bm += c * wt;
     }
-    __syncthreads();
-    if (threadIdx.x >= 32) return;
-    // the thread's places, a pair per lane
-    const int lane = threadIdx.x;
-    int c0 = 0, c1 = 0;
-    double w0 = 0.0, w1 = 0.0;
-    const int m = (rank * SQ_NT + t) * pairs + lane;
-    if (lane < pairs) {
-      pair(m, &c0, &c1);
-      if (c0) w0 = weight(2 * m);
-      if (c1) w1 = weight(2 * m + 1);
-    }
-    const double m0 = c0 * w0, m1 = c1 * w1;
-    const int en = s.before_n + sp_warp_scan(c0 + c1);
-    const double em = s.before_m + sp_warp_scan(m0 + m1);
-    const uint32_t yes = __ballot_sync(0xffffffffu, (c0 | c1) && past(en, em)),
-                   any = __ballot_sync(0xffffffffu, (c0 | c1) != 0);
-    const int l = yes ? __ffs(yes) - 1 : 31 - __clz(any);
-    if (lane != l) return;
-    const int b0 = en - c0 - c1;
-    const double a0 = em - (m0 + m1);
-    const bool second = !c0 || (c1 && !past(b0 + c0, a0 + m0));
-    const int bn = second ? b0 + c0 : b0, c = second ? c1 : c0;
-    const double bm = second ? a0 + m0 : a0, wt = second ? w1 : w0;
-    // values of the place before the crossing: the least j with past(bn + j + 1, ...)
+    // the least j with past(bn + j + 1, ...)
     int lo = 0, hi = c - 1;
     while (lo < hi) {
       const int j = (lo + hi) / 2;
       if (past(bn + j + 1, bm + (j + 1.0) * wt)) hi = j;
       else lo = j + 1;
     }
-    const SqHit h{bn + lo + 1, lo, 2 * m + (second ? 1 : 0), bm + (lo + 1.0) * wt};
-    for (int r = 0; r < ranks; ++r) of(s, r).hit[w] = h;
+    const SqHit h{bn + lo + 1, lo, place, bm + (lo + 1.0) * wt};
+#pragma unroll
+    for (int r = 0; r < RANKS; ++r) of(s, r).hit[w] = h;
   }
 };
 
-template <typename E>
+template <typename E, int RANKS>
 __global__ void __launch_bounds__(SQ_NT, 1) sample_min_p16_kernel(const SpArgs a) {
   __shared__ SqShared s;
-  SqRow<E> R{cg::this_cluster()};
+  using Row = SqRow<E, RANKS>;
+  Row R{cg::this_cluster()};
   R.rank = (int)R.cl.block_rank();
-  R.ranks = (int)R.cl.num_blocks();
-  R.pairs = SQ_CODES / 2 / R.ranks;
-  const int row = blockIdx.x / R.ranks, t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int row = blockIdx.x / RANKS, t = threadIdx.x, lane = t & 31, warp = t >> 5;
   SpOptions o;
   if (!o.read(a, row)) {
     if (R.rank == 0 && t == 0) sp_write_bad(a, row, NCB_FLAG_BAD_OPTIONS);
@@ -1488,42 +1467,88 @@ __global__ void __launch_bounds__(SQ_NT, 1) sample_min_p16_kernel(const SpArgs a
   }
   R.cl.sync();
 
-  // ---- this thread's places: counts, then masses -----------------------------------------------
-  // Neighbouring lanes start at different words, so that they read different banks.
-  const int turn = lane * R.pairs / 32, m0 = (R.rank * SQ_NT + t) * R.pairs;
-  int first = 65536, bad = 0;
-  uint32_t filled = 0;  // pairs with a value
-  R.n = 0;
-  for (int i = 0; i < R.pairs; ++i) {
-    const int j = (i + turn) & (R.pairs - 1), m = m0 + j;
-    int c0, c1;
-    R.pair(m, &c0, &c1);
-    if (c0 | c1) {
-      R.n += c0 + c1;
-      filled |= 1u << j;
-      first = min(first, c0 ? 2 * m : 2 * m + 1);
-      const uint32_t b0 = sq_bits(2 * m), b1 = sq_bits(2 * m + 1);
-      bad |= (c0 && (b0 & 0x7FFFu) >= SqType<E>::INF) || (c1 && (b1 & 0x7FFFu) >= SqType<E>::INF);
+  // ---- this thread's places, over the cluster ----------------------------------------------------
+  // Places 2 m and 2 m + 1 share a counter word; of the positive values the words (and
+  // in a word the halves) are in falling order of places. Read by 16 bytes, neighbouring
+  // lanes starting at different ones, so that they read different banks (by 4 bytes the
+  // other CTAs' words took 20 us).
+  constexpr int VECS = Row::PAIRS / 4;
+  const int m0 = (R.rank * SQ_NT + t) * Row::PAIRS, turn = lane * VECS / 8;
+  const int block = (m0 < 16384 ? 16384 - m0 - Row::PAIRS : m0) / 4;
+  int lo[Row::PAIRS], hi[Row::PAIRS];
+#pragma unroll
+  for (int v = 0; v < VECS; ++v) {
+    uint4* from = sp_raw + block + ((v + turn) & (VECS - 1));
+#pragma unroll
+    for (int c = 0; c < 4; ++c) lo[4 * v + c] = hi[4 * v + c] = 0;
+#pragma unroll
+    for (int r = 0; r < RANKS; ++r) {
+      const uint4 x = RANKS == 1 ? *from : *R.cl.map_shared_rank(from, r);
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if constexpr (RANKS == 1) {
+          lo[4 * v + c] = (int)w[c];  // both, to be taken apart
+        } else {
+          lo[4 * v + c] += (int)(w[c] & 0xFFFFu);
+          hi[4 * v + c] += (int)(w[c] >> 16);
+        }
+      }
     }
   }
+  const bool down = m0 < 16384;
+  auto pair_of = [&](int j) {  // which of the thread's pairs of places it is
+    const int q = (((j >> 2) + turn) & (VECS - 1)) * 4 + (j & 3);
+    return down ? Row::PAIRS - 1 - q : q;
+  };
+  auto counts_of = [&](int j, int* c0, int* c1) {
+    const int l = RANKS == 1 ? (int)((uint32_t)lo[j] & 0xFFFFu) : lo[j],
+              h = RANKS == 1 ? (int)((uint32_t)lo[j] >> 16) : hi[j];
+    *c0 = down ? h : l;
+    *c1 = down ? l : h;
+  };
+  unsigned long long filled = 0;  // by place within the thread's
+  R.n = 0;
+#pragma unroll
+  for (int j = 0; j < Row::PAIRS; ++j) {
+    if (RANKS == 1 ? lo[j] == 0 : (lo[j] | hi[j]) == 0) continue;
+    int c0, c1;
+    counts_of(j, &c0, &c1);
+    R.n += c0 + c1;
+    filled |= (unsigned long long)((c0 ? 1 : 0) | (c1 ? 2 : 0)) << (2 * pair_of(j));
+  }
+  // Not finite: places of +NaN and +inf come first, those of -NaN last.
+  constexpr int P_FIRST = 32768 - (int)SqType<E>::INF, P_LAST = 32768 + (int)SqType<E>::INF - 1;
+  const int p0 = 2 * m0;
+  int first = 65536, bad = 0;
+  if (filled) {
+    first = p0 + __ffsll((long long)filled) - 1;
+    const int last = p0 + 63 - __clzll((long long)filled);
+    bad = first < P_FIRST || last > P_LAST;
+  }
+  const int nz = __popcll(filled), nz_in = sp_warp_scan(nz);
   {
     const int wn = __reduce_add_sync(0xffffffffu, R.n), wf = __reduce_min_sync(0xffffffffu, first);
     if (lane == 0) s.red_i[warp] = wn, s.in_warp[0][warp] = wf;
+    if (lane == 31) s.red_j[warp] = nz_in;
     bad = __syncthreads_or(bad);
     if (t < 32) {
       const int cn = __reduce_add_sync(0xffffffffu, s.red_i[t]),
-                cf = __reduce_min_sync(0xffffffffu, s.in_warp[0][t]);
-      if (t < R.ranks) {
+                cf = __reduce_min_sync(0xffffffffu, s.in_warp[0][t]), nz_w = sp_warp_scan(s.red_j[t]);
+      s.in_warp[1][t] = nz_w - s.red_j[t];
+      if (t == 31) s.at = nz_w;
+      if (t < RANKS) {
         SqShared& to = R.of(s, t);
         to.tot_n[R.rank] = cn;
         to.first[R.rank] = cf;
         to.bad[R.rank] = bad;
       }
     }
-    R.cl.sync();
+    R.cl.sync();  // the counters are not read any more
   }
   int total = 0, top = 65536;
-  for (int r = 0; r < R.ranks; ++r) {
+#pragma unroll
+  for (int r = 0; r < RANKS; ++r) {
     total += s.tot_n[r];
     top = min(top, s.first[r]);
     bad |= s.bad[r];
@@ -1537,29 +1562,68 @@ __global__ void __launch_bounds__(SQ_NT, 1) sample_min_p16_kernel(const SpArgs a
   int many = 1;
   double left = 1.0;
   R.k.mx = mx;
+  // ---- the list ---------------------------------------------------------------------------------
+  R.entries = s.at;
+  {
+    const int at = s.in_warp[1][warp] + nz_in - nz;
+#pragma unroll
+    for (int j = 0; j < Row::PAIRS; ++j) {
+      if (RANKS == 1 ? lo[j] == 0 : (lo[j] | hi[j]) == 0) continue;
+      int c0, c1;
+      counts_of(j, &c0, &c1);
+      const int b = 2 * pair_of(j);
+      const int i = at + __popcll(filled & ((1ull << b) - 1));
+      const uint32_t place = (uint32_t)(2 * Row::PAIRS * t + b);
+      if (c0) R.counts()[i] = (uint32_t)c0 * Row::PLACES | place;
+      if (c1) R.counts()[i + (c0 ? 1 : 0)] = (uint32_t)c1 * Row::PLACES | (place + 1);
+    }
+  }
   if (!greedy) {
     R.k.inv_t = 1.0 / (double)o.T;
     R.k.c = R.k.inv_t / 0.69314718055994530942;
     const double far = (double)mx - SP_REACH * (double)o.T;
     R.k.zero = far > -(double)FLT_MAX ? (float)far : -FLT_MAX;
+    if (t == 0) s.theta = sp_least_kept(mx, o.T, o.min_p, R.k.inv_t);
+  }
+  __syncthreads();
+  if (!greedy) {
+    // ---- masses: of this thread's entries, before them, of the CTA's, and what min-p keeps -----------
+    R.per = (R.entries + SQ_NT - 1) / SQ_NT;
+    const float theta = s.theta;
+    R.n = 0;
     R.mass = 0.0;
-    for (int i = 0; i < R.pairs; ++i) {
-      const int j = (i + turn) & (R.pairs - 1), m = m0 + j;
-      if (!(filled >> j & 1)) continue;
-      int c0, c1;
-      R.pair(m, &c0, &c1);
-      R.mass += c0 * R.weight(2 * m) + c1 * R.weight(2 * m + 1);
+    int kept_n = 0;
+    double kept_m = 0.0;
+    for (int i = t * R.per; i < min(R.entries, (t + 1) * R.per); ++i) {
+      const uint32_t e = R.counts()[i];
+      const int place = R.place_of(e), c = R.count_of(e);
+      const double m = c * R.weight(place);
+      R.n += c;
+      R.mass += m;
+      if (SqType<E>::value(sq_bits(place)) >= theta) kept_n += c, kept_m += m;
     }
-    // prefixes over the CTA's threads
     const int in = sp_warp_scan(R.n);
     const double im = sp_warp_scan(R.mass);
-    if (lane == 31) s.red_i[warp] = in, s.red_d[warp] = im;
+    kept_n = __reduce_add_sync(0xffffffffu, kept_n);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) kept_m += __shfl_xor_sync(0xffffffffu, kept_m, x);
+    if (lane == 31) s.red_i[warp] = in, s.red_d[warp] = im, s.red_j[warp] = kept_n, s.red_e[warp] = kept_m;
     __syncthreads();
     if (t < 32) {
       const int wn = sp_warp_scan(s.red_i[t]);
       const double wm = sp_warp_scan(s.red_d[t]);
+      const int kn = __reduce_add_sync(0xffffffffu, s.red_j[t]);
+      double km = s.red_e[t];
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) km += __shfl_xor_sync(0xffffffffu, km, x);
       if (t == 31)
-        for (int r = 0; r < R.ranks; ++r) R.of(s, r).tot_m[R.rank] = wm;
+#pragma unroll
+        for (int r = 0; r < RANKS; ++r) {
+          SqShared& to = R.of(s, r);
+          to.tot_m[R.rank] = wm;
+          to.kept_n[R.rank] = kn;
+          to.kept_m[R.rank] = km;
+        }
       s.red_i[t] = wn - s.red_i[t];
       s.red_d[t] = wm - s.red_d[t];
     }
@@ -1568,51 +1632,24 @@ __global__ void __launch_bounds__(SQ_NT, 1) sample_min_p16_kernel(const SpArgs a
     R.before_m = s.red_d[warp] + (im - R.mass);
     R.cl.sync();
 
-    // ---- K, and what min-p keeps ---------------------------------------------------------------
+    // ---- K, P, what min-p keeps, and the draw ------------------------------------------------------
     const int kk = o.top_k > 0 && o.top_k < total ? o.top_k : total;
-    double mass = 0.0;
-    for (int r = 0; r < R.ranks; ++r) mass += s.tot_m[r];
-    many = kk;
-    if (kk < total) R.cross(s, SP_K, [&](int n, double) { return n >= kk; });
-    if (o.min_p > 0.0f) {
-      __syncthreads();
-      if (t == 0) s.before_m = (double)sp_least_kept(mx, o.T, o.min_p, R.k.inv_t);
-      __syncthreads();
-      const float least = (float)s.before_m;
-      __syncthreads();
-      // the CTA that owns the last place at or above it adds up: places before the
-      // thread's, and the thread's own
-      int pn = 0;
-      double pm = 0.0;
-      for (int i = 0; i < R.pairs; ++i) {
-        if (!(filled >> i & 1)) continue;
-        int c0, c1;
-        R.pair(m0 + i, &c0, &c1);
-        if (c0 && SqType<E>::value(sq_bits(2 * (m0 + i))) >= least) pn += c0, pm += c0 * R.weight(2 * (m0 + i));
-        if (c1 && SqType<E>::value(sq_bits(2 * (m0 + i) + 1)) >= least) pn += c1, pm += c1 * R.weight(2 * (m0 + i) + 1);
-      }
-      pn = __reduce_add_sync(0xffffffffu, pn);
+    int pn = 0;
+    double pm = 0.0;
 #pragma unroll
-      for (int x = 16; x > 0; x >>= 1) pm += __shfl_xor_sync(0xffffffffu, pm, x);
-      if (lane == 0) s.red_i[warp] = pn, s.red_d[warp] = pm;
-      __syncthreads();
-      if (t < 32) {
-        pn = __reduce_add_sync(0xffffffffu, s.red_i[t]);
-        pm = s.red_d[t];
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) pm += __shfl_xor_sync(0xffffffffu, pm, x);
-        if (t < R.ranks) {
-          R.of(s, t).found[R.rank] = pn;
-          R.of(s, t).kept_m[R.rank] = pm;
-        }
-      }
+    for (int r = 0; r < RANKS; ++r) {
+      left = r ? left + s.tot_m[r] : s.tot_m[r];
+      pn += s.kept_n[r];
+      pm += s.kept_m[r];
     }
-    if (kk < total || o.min_p > 0.0f) R.cl.sync();
-    if (kk < total) mass = s.hit[SP_K].mass;
-    // ---- P ------------------------------------------------------------------------------------------
-    left = mass;
+    many = kk;
+    if (kk < total) {
+      R.cross(s, SP_K, [&](int n, double) { return n >= kk; });
+      R.cl.sync();
+      left = s.hit[SP_K].mass;
+    }
     if (o.top_p < 1.0f) {
-      const double want = (double)o.top_p * mass;
+      const double want = (double)o.top_p * left;
       R.cross(s, SP_P, [&](int, double x) { return x >= want; });
       R.cl.sync();
       if (s.hit[SP_P].n < many) {
@@ -1620,16 +1657,7 @@ __global__ void __launch_bounds__(SQ_NT, 1) sample_min_p16_kernel(const SpArgs a
         left = s.hit[SP_P].mass;
       }
     }
-    if (o.min_p > 0.0f) {
-      int pn = 0;
-      double pm = 0.0;
-      for (int r = 0; r < R.ranks; ++r) {
-        pn += s.found[r];
-        pm += s.kept_m[r];
-      }
-      if (pn < many) many = pn, left = pm;
-    }
-    // ---- the draw -------------------------------------------------------------------------------------
+    if (pn < many) many = pn, left = pm;
     const double want = (double)o.u * left;
     R.cross(s, SP_D, [&](int n, double x) { return x > want || n >= many; });
     R.cl.sync();
@@ -1639,10 +1667,21 @@ __global__ void __launch_bounds__(SQ_NT, 1) sample_min_p16_kernel(const SpArgs a
   // ---- the token: the nth value at the place, by id --------------------------------------------------
   const float value = SqType<E>::value(sq_bits(draw.place));
   int nth = draw.nth;
-  if (draw.place == 32768) {  // -0: as good as +0, whose values come before
-    int c0, plus;
-    R.pair(16383, &c0, &plus);
-    nth += plus;
+  if (draw.place == 32768 && !greedy) {  // -0: as good as +0, whose values come before
+    __syncthreads();
+    if (t == 0) s.at = 0;
+    __syncthreads();
+    if (R.rank == (32767 / Row::PLACES))
+      for (int i = t; i < R.entries; i += SQ_NT)
+        if (R.place_of(R.counts()[i]) == 32767) s.at = R.count_of(R.counts()[i]);
+    __syncthreads();
+    if (RANKS > 1) {
+      if (R.rank == (32767 / Row::PLACES) && t < RANKS) R.of(s, t).first[0] = s.at;
+      R.cl.sync();
+      nth += s.first[0];
+    } else {
+      nth += s.at;
+    }
   }
   const uint32_t want = sq_bits(draw.place), also = value == 0.0f ? want ^ 0x8000u : want;
   auto matches = [&](const uint4& g) {  // bit e: value e of the granule is it
@@ -1674,8 +1713,8 @@ __global__ void __launch_bounds__(SQ_NT, 1) sample_min_p16_kernel(const SpArgs a
     if (w < warp) before += s.red_i[w];
     here += s.red_i[w];
   }
-  if (R.ranks > 1) {
-    if (t < R.ranks) R.of(s, t).here[R.rank] = here;
+  if (RANKS > 1) {
+    if (t < RANKS) R.of(s, t).here[R.rank] = here;
     R.cl.sync();
     for (int r = 0; r < R.rank; ++r) before += s.here[r];
   }
@@ -1730,21 +1769,25 @@ int sp_launch(const nvs::SpArgs& a, int rows, int device, int num_sms, cudaStrea
   const int granules = (a.vocab + n - 1) / n + 1;
   if constexpr (sizeof(E) == 2) {
     // as many CTAs to a row as its values need, then as fill the GPU, one per SM
-    int ranks = 1;
+    const int values = granules * n;
+    int ranks = values <= nvs::SQ_ALONE ? 1 : 2;
     while (ranks < nvs::SP_CLUSTER &&
            ((granules + ranks - 1) / ranks * n > nvs::SQ_SLICE ||
             ((int64_t)rows * ranks * 2 <= num_sms && granules / ranks >= 2 * nvs::SQ_NT)))
       ranks *= 2;
     if ((granules + ranks - 1) / ranks * n <= nvs::SQ_SLICE) {
       constexpr int smem = 65536 * 2;
-      static std::atomic<bool> raised[SP_DEVICES];  // per device; raising it twice is harmless
-      if (device >= SP_DEVICES || !raised[device].load(std::memory_order_acquire)) {
-        if (cudaFuncSetAttribute(nvs::sample_min_p16_kernel<E>,
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+      const auto kernel = ranks == 1   ? nvs::sample_min_p16_kernel<E, 1>
+                          : ranks == 2 ? nvs::sample_min_p16_kernel<E, 2>
+                          : ranks == 4 ? nvs::sample_min_p16_kernel<E, 4>
+                                       : nvs::sample_min_p16_kernel<E, 8>;
+      static std::atomic<int> raised[SP_DEVICES];  // per device, a bit per kernel; twice is harmless
+      if (device >= SP_DEVICES || !(raised[device].load(std::memory_order_acquire) & ranks)) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
           return NCB_ERROR_LAUNCH_FAILED;
-        if (device < SP_DEVICES) raised[device].store(true, std::memory_order_release);
+        if (device < SP_DEVICES) raised[device].fetch_or(ranks, std::memory_order_release);
       }
-      return sp_start(nvs::sample_min_p16_kernel<E>, a, rows, granules, ranks, nvs::SQ_NT, smem, st);
+      return sp_start(kernel, a, rows, granules, ranks, nvs::SQ_NT, smem, st);
     }
   }
   // as many CTAs to a row as fill the GPU twice over, while each has two granules for

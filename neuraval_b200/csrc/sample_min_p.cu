@@ -53,6 +53,7 @@ constexpr int SP_FEW = 1024;     // values that one list holds and sorts
 constexpr int SP_CAP = 512;      // and one window's part of the list
 constexpr int SP_WIDEN = 96;     // values up to which a guessed window takes in its neighbours
 constexpr int SP_RANKED = 256;   // lists up to this are sorted by ranks
+constexpr int SP_SOME = 512;     // bins of which a value is kept, for the guess
 constexpr int SP_BOUNDED = 256;  // largest top_k that the threads' maxima bound
 constexpr int SP_CLUSTER = 8;    // largest cluster
 constexpr int SP_TURNS = 4096;   // passes over a row at most
@@ -83,10 +84,10 @@ enum { SP_K = 0, SP_P = 1, SP_D = 2, SP_WINDOWS = 3 };
 
 struct SpCmd {
   int op;
-  float above[SP_WINDOWS], below[SP_WINDOWS];  // SP_FIRST: each window's bins, [above, below)
+  float high[SP_WINDOWS], low[SP_WINDOWS];  // SP_FIRST: each window's values, both ends in it
   uint32_t klo[SP_WINDOWS], khi[SP_WINDOWS];  // each window's keys, both ends in it
   int gather[SP_WINDOWS];                     // whether its values are listed
-  float theta;                                // least value that min-p keeps
+  float theta;                                // least value that min-p keeps; SP_GATHER: least wanted
   int shift;                                  // SP_HIST: bin = (khi[0] - key) >> shift; < 0: bin(value)
   float value;                                // SP_SELECT: the value and which of its
   int nth;                                    //   occurrences, by id
@@ -106,7 +107,7 @@ struct SpPart {
 
 struct SpShared {
   uint4 hist4[SP_BINS / 4];  // counts; in CTA 0, once merged, the counts before each bin
-  float4 some4[SP_BINS / 4]; // a value of each filled bin
+  float4 some4[SP_SOME / 4]; // a value of each filled bin, of the first bins
   alignas(16) float mass[SP_BINS + 4];  // CTA 0, once merged: about the mass before each bin
   unsigned long long list[SP_WINDOWS * SP_CAP];
   SpCmd cmd;
@@ -125,7 +126,7 @@ struct SpShared {
   double got_d;
   int got_i, bin_k, bin_last;
   float theta;
-  uint32_t tops[2];
+  uint32_t tops[2 * SP_WINDOWS];
 };
 
 // The CTA's shared memory, by a name that is known to be shared: through a pointer in
@@ -140,6 +141,11 @@ __device__ __forceinline__ uint32_t sp_key(float v) {
 }
 __device__ __forceinline__ float sp_value(uint32_t k) {
   return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+}
+// A window's greatest key as a value. (No value has the key of -0; as a float it would
+// take +0 with it.)
+__device__ __forceinline__ float sp_edge(uint32_t k) {
+  return sp_value(k == 0x7FFFFFFFu ? 0x7FFFFFFEu : k);
 }
 __device__ __forceinline__ float sp_max_nan(float a, float b) {
   float r;
@@ -454,7 +460,7 @@ struct SpRow {
         if (v[e] > -INFINITY) {
           const int b = k.bin(v[e]);
           atomicAdd(reinterpret_cast<int*>(s.hist4) + b, 1);
-          reinterpret_cast<float*>(s.some4)[b] = v[e];  // any of them, for the guess alone
+          if (b < SP_SOME) reinterpret_cast<float*>(s.some4)[b] = v[e];  // any of them
         }
     });
   }
@@ -467,7 +473,6 @@ struct SpRow {
         if (k >= m.klo[0] && k <= m.khi[0]) {
           const uint32_t b = (m.khi[0] - k) >> m.shift;
           atomicAdd(reinterpret_cast<int*>(s.hist4) + b, 1);
-          reinterpret_cast<float*>(s.some4)[b] = v[e];
         }
       }
     });
@@ -480,13 +485,17 @@ struct SpRow {
   }
   __device__ __noinline__ void gather(const SpCmd& m) {
     SpShared& s = sp_shared();
-    const SpView k = this->k;
     SpShared& to = of(0);
-    const float below = m.below[0];
-    sl.template each<2>([&](const float* v, int i) {
+    const float least = m.theta;
+    sl.template each<4>([&](const float* v, int i) {
+      float most = v[0];
 #pragma unroll
-      for (int e = 0; e < SpVec<E>::N; ++e)
-        if (k.place(v[e]) < below && v[e] > -INFINITY) put(to, 0, 0, SP_FEW, v[e], sl.id(i, e));
+      for (int e = 1; e < SpVec<E>::N; ++e) most = fmaxf(most, v[e]);
+      if (most >= least) {
+#pragma unroll
+        for (int e = 0; e < SpVec<E>::N; ++e)
+          if (v[e] >= least) put(to, 0, 0, SP_FEW, v[e], sl.id(i, e));
+      }
     });
   }
   // The usual pass: windows that are runs of bins. Exact masses above each and of what
@@ -496,13 +505,14 @@ struct SpRow {
     SpShared& s = sp_shared();
     const SpView k = this->k;
     SpShared& to = of(0);
-    float above[SP_WINDOWS], below[SP_WINDOWS];
+    float lo[SP_WINDOWS], hi[SP_WINDOWS];
 #pragma unroll
     for (int w = 0; w < SP_WINDOWS; ++w) {
-      above[w] = m.above[w];
-      below[w] = m.below[w];
+      lo[w] = m.low[w];
+      hi[w] = m.high[w];
     }
     const float theta = m.theta;
+    const bool all = theta == -FLT_MAX;  // min-p keeps all: their mass is not asked for
     double mass[SP_WINDOWS + 1] = {};
     uint32_t low[SP_WINDOWS], high[SP_WINDOWS];
 #pragma unroll
@@ -511,22 +521,24 @@ struct SpRow {
     sl.template each<1>([&](const float* v, int i) {
 #pragma unroll
       for (int e = 0; e < SpVec<E>::N; ++e) {
-        const float x = v[e], q = k.place(x);
+        const float x = v[e];
         // out of reach: weighed as if just within it, and not added
         const double wt = k.weight(fmaxf(x, k.zero));
         const bool near = x >= k.zero;
         bool in = false;
 #pragma unroll
         for (int w = 0; w < SP_WINDOWS; ++w) {
-          if (near && q < above[w]) mass[w] += wt;
-          in |= q >= above[w] && q < below[w];
+          if (near && x > hi[w]) mass[w] += wt;
+          in |= x <= hi[w] && x >= lo[w];
         }
-        if (near && x >= theta) mass[SP_WINDOWS] += wt;
-        n += x >= theta;
-        if (in && x > -INFINITY) {
+        if (!all) {
+          if (near && x >= theta) mass[SP_WINDOWS] += wt;
+          n += x >= theta;
+        }
+        if (in) {
 #pragma unroll
           for (int w = 0; w < SP_WINDOWS; ++w)
-            if (q >= above[w] && q < below[w]) {
+            if (x <= hi[w] && x >= lo[w]) {
               if (m.gather[w]) {
                 put(to, w, w * SP_CAP, SP_CAP, x, sl.id(i, e));
               } else {
@@ -588,8 +600,7 @@ struct SpRow {
 #pragma unroll
     for (int w = 0; w < SP_WINDOWS; ++w) {
       lo[w] = sp_value(m.klo[w]);
-      // no value has the key of -0; as a float it would take +0 with it
-      hi[w] = sp_value(m.khi[w] == 0x7FFFFFFFu ? 0x7FFFFFFEu : m.khi[w]);
+      hi[w] = sp_edge(m.khi[w]);
     }
     SpPart p{};
     sl.template each<1>([&](const float* v, int i) {
@@ -704,11 +715,10 @@ struct SpRow {
 
   // ---- CTA 0 ----------------------------------------------------------------------
   // The cluster's counts added up: hist4 becomes the counts before each bin, mass
-  // about the mass before each bin: n_b times the weight at the bin's centre, or of a
-  // value in it where that is the only one, or where the type has few values (16 bits:
-  // a bin mostly holds one value many times).
+  // about the mass before each bin: n_b times the weight at the bin's centre, or, in the
+  // first bins by value, which hold few values and most of the mass, of a value in it.
   template <typename F>
-  __device__ __noinline__ int merge(F centre) {
+  __device__ __noinline__ int merge(F centre, bool by_value) {
     SpShared& s = sp_shared();
     int n[4] = {0, 0, 0, 0};
     float x[4];
@@ -716,7 +726,8 @@ struct SpRow {
     for (int r = 0; r < SP_CLUSTER; ++r)
       if (r < ranks) {
         const uint4 c = of(r).hist4[threadIdx.x];
-        const float4 f = of(r).some4[threadIdx.x];
+        const float4 f = by_value && 4 * threadIdx.x < SP_SOME ? of(r).some4[threadIdx.x]
+                                                              : make_float4(0.f, 0.f, 0.f, 0.f);
         const uint32_t ci[4] = {c.x, c.y, c.z, c.w};
         const float fi[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
@@ -732,8 +743,8 @@ struct SpRow {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       m[j] = !n[j] ? 0.f
-             : n[j] == 1 || sizeof(E) == 2 ? n[j] * __expf((x[j] - k.mx) * rate)
-                                           : n[j] * centre(b + j);
+             : by_value && b < SP_SOME ? n[j] * __expf((x[j] - k.mx) * rate)
+                                       : n[j] * centre(b + j);
       mi += m[j];
       ni += n[j];
     }
@@ -916,7 +927,7 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
   s.hist4[t] = make_uint4(0, 0, 0, 0);
   if (t < SP_WINDOWS) s.n_list[t] = 0;
   float mx = -INFINITY, mn = INFINITY;
-  R.sl.template each<2>([&](const float* v, int) {
+  R.sl.template each<4>([&](const float* v, int) {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
       mx = sp_max_nan(mx, v[e]);
@@ -993,14 +1004,17 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
   if (few) {
     int deep = SP_BINS - 1;  // the last bin that has to be known
     if (bounded) {
-      const int maxima = R.merge(centre);
+      const int maxima = R.merge(centre, false);
       if (maxima >= k_asked) deep = R.bin_of_count(k_asked, maxima);
     }
     __syncthreads();
     if (min_p > 0.0f && top_p >= 1.0f) deep = min(deep, R.k.bin(s.theta));
     if (t == 0) {
       s.cmd.op = SP_GATHER;
-      s.cmd.below[0] = deep == SP_BINS - 1 ? INFINITY : (float)(deep + 1);
+      // not above any value of these bins, whose places are off by 2^-23 of them at most
+      const double edge = (double)mx - (deep + 1) / (double)R.k.scale * (1.0 + 1e-6);
+      s.cmd.theta = deep == SP_BINS - 1 || !(edge > -(double)FLT_MAX) ? -FLT_MAX
+                                                                     : nextafterf((float)edge, -INFINITY);
     }
     R.command();
     const int n = s.n_list[0];
@@ -1019,7 +1033,7 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
     }
     R.command();
   }
-  const int total = R.merge(centre);
+  const int total = R.merge(centre, true);
   const int k = k_asked > 0 && k_asked < total ? k_asked : total;
   const int bk = R.bin_of_count(k, total);
   const float theta = s.theta;  // (written before merge's barriers)
@@ -1031,7 +1045,7 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
     // ---- few: one list decides ---------------------------------------------------------
     if (t == 0) {
       s.cmd.op = SP_GATHER;
-      s.cmd.below[0] = deep == SP_BINS - 1 ? INFINITY : (float)(deep + 1);
+      s.cmd.theta = sp_value(R.top_of_bin(deep + 1) + 1);
       s.n_list[0] = 0;
     }
     R.command();
@@ -1075,21 +1089,25 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
       s.cmd.shift = -1;
     }
     R.command();
-    R.merge(centre);
+    R.merge(centre, true);
     by_value = true;
   };
-  // A window of bins: listed where it fits, and its keys, which only the general pass
-  // asks for.
+  // A window of bins is listed where it fits; then, of all such, the keys.
   auto set_bins = [&](int w) {
     win[w].by_key = win[w].weigh = false;
     win[w].gather = R.before(win[w].z + 1, total) - R.before(win[w].a, total) <= SP_CAP;
   };
-  auto set_keys = [&](int w) {
-    if (t < 2) s.tops[t] = R.top_of_bin(t == 0 ? win[w].a : win[w].z + 1);
+  auto set_keys = [&] {
     __syncthreads();
-    win[w].khi = s.tops[0];
-    win[w].klo = s.tops[1] + 1;
+    for (int w = 0; w < SP_WINDOWS; ++w)
+      if (!found[w] && !win[w].by_key && (t == 32 * w || t == 32 * w + SP_NT / 2))
+        s.tops[t == 32 * w ? w : SP_WINDOWS + w] = R.top_of_bin(t == 32 * w ? win[w].a : win[w].z + 1);
     __syncthreads();
+    for (int w = 0; w < SP_WINDOWS; ++w)
+      if (!found[w] && !win[w].by_key) {
+        win[w].khi = s.tops[w];
+        win[w].klo = s.tops[SP_WINDOWS + w] + 1;
+      }
   };
   for (int w = 0; w < SP_WINDOWS; ++w)
     if (!found[w]) set_bins(w);
@@ -1112,7 +1130,7 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
     const int n = R.merge([&](int b) {
       const uint32_t key = hi - min(((uint32_t)b << shift) + half, hi - lo);
       return (float)R.k.weight_any(sp_value(key));
-    });
+    }, false);
     int a1, z1;
     if (count) {
       a1 = z1 = R.bin_of_count((int)want - n_above, n);
@@ -1137,9 +1155,7 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
   for (int turn = 0; !found[SP_D] && turn < SP_TURNS; ++turn) {
     bool first = true;  // all windows are runs of bins: the first pass will do
     for (int w = 0; w < SP_WINDOWS; ++w) first = first && (found[w] || !(win[w].by_key || win[w].weigh));
-    if (!first)
-      for (int w = 0; w < SP_WINDOWS; ++w)
-        if (!found[w] && !win[w].by_key) set_keys(w);
+    set_keys();
     if (first) need_bins();
     if (t == 0) {
       s.cmd.op = first ? SP_FIRST : SP_PASS;
@@ -1147,8 +1163,8 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
       for (int w = 0; w < SP_WINDOWS; ++w) {
         // a window that is not looked at any more: nothing in it, and above it every
         // value for K (whose mass is then the row's), none for the others
-        s.cmd.above[w] = found[w] ? (w == SP_K ? INFINITY : 0.0f) : (float)win[w].a;
-        s.cmd.below[w] = found[w] ? 0.0f : win[w].z == SP_BINS - 1 ? INFINITY : (float)(win[w].z + 1);
+        s.cmd.high[w] = found[w] ? (w == SP_K ? -INFINITY : INFINITY) : sp_edge(win[w].khi);
+        s.cmd.low[w] = found[w] ? INFINITY : sp_value(win[w].klo);
         s.cmd.klo[w] = found[w] ? 0xFFFFFFFFu : win[w].klo;
         s.cmd.khi[w] = found[w] ? (w == SP_K ? sp_key(-INFINITY) : sp_key(INFINITY)) : win[w].khi;
         s.cmd.gather[w] = !found[w] && win[w].gather;
@@ -1267,7 +1283,7 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
     }
     many = n_p;
     left = mass_p;
-    if (p.n_above(SP_WINDOWS) < many) {
+    if (theta > -FLT_MAX && p.n_above(SP_WINDOWS) < many) {
       many = p.n_above(SP_WINDOWS);
       left = p.above(SP_WINDOWS);
     }

@@ -501,6 +501,8 @@ struct SpRow {
   // The usual pass: windows that are runs of bins. Exact masses above each and of what
   // min-p keeps; the values of a window into its list, or, where they are too many,
   // their least and greatest key (they may all be one value).
+  // WITH_K: K's mass ends at a window too (otherwise it is the row's); WITH_M: min-p is on.
+  template <bool WITH_K, bool WITH_M>
   __device__ __noinline__ void first_pass(const SpCmd& m) {
     SpShared& s = sp_shared();
     const SpView k = this->k;
@@ -512,30 +514,45 @@ struct SpRow {
       hi[w] = m.high[w];
     }
     const float theta = m.theta;
-    const bool all = theta == -FLT_MAX;  // min-p keeps all: their mass is not asked for
     double mass[SP_WINDOWS + 1] = {};
     uint32_t low[SP_WINDOWS], high[SP_WINDOWS];
 #pragma unroll
     for (int w = 0; w < SP_WINDOWS; ++w) low[w] = 0xFFFFFFFFu, high[w] = 0;
     int n = 0;
     sl.template each<1>([&](const float* v, int i) {
+      uint32_t in = 0;  // values of the granule in some window
 #pragma unroll
-      for (int e = 0; e < SpVec<E>::N; ++e) {
-        const float x = v[e];
-        // out of reach: weighed as if just within it, and not added
-        const double wt = k.weight(fmaxf(x, k.zero));
-        const bool near = x >= k.zero;
-        bool in = false;
+      for (int e0 = 0; e0 < SpVec<E>::N; e0 += 2) {
+        double wt[2];  // two at a time: each is a long chain of 64-bit operations
 #pragma unroll
-        for (int w = 0; w < SP_WINDOWS; ++w) {
-          if (near && x > hi[w]) mass[w] += wt;
-          in |= x <= hi[w] && x >= lo[w];
+        for (int h = 0; h < 2; ++h) {
+          // out of reach: weighed as if just within it, and not added
+          const float x = v[e0 + h];
+          wt[h] = k.weight(fmaxf(x, k.zero));
+          if (!(x >= k.zero)) wt[h] = 0.0;
         }
-        if (!all) {
-          if (near && x >= theta) mass[SP_WINDOWS] += wt;
-          n += x >= theta;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float x = v[e0 + h];
+          bool at = false;
+#pragma unroll
+          for (int w = WITH_K ? SP_K : SP_P; w < SP_WINDOWS; ++w) {
+            if (x > hi[w]) mass[w] += wt[h];
+            at |= x <= hi[w] && x >= lo[w];
+          }
+          if (!WITH_K) mass[SP_K] += wt[h];
+          if (at) in |= 1u << (e0 + h);
+          if (WITH_M && x >= theta) {
+            mass[SP_WINDOWS] += wt[h];
+            ++n;
+          }
         }
-        if (in) {
+      }
+      if (in) {
+#pragma unroll
+        for (int e = 0; e < SpVec<E>::N; ++e) {
+          if (!(in >> e & 1)) continue;
+          const float x = v[e];
 #pragma unroll
           for (int w = 0; w < SP_WINDOWS; ++w)
             if (x <= hi[w] && x >= lo[w]) {
@@ -677,7 +694,11 @@ struct SpRow {
   }
   __device__ __noinline__ void carry_out(const SpCmd& m) {
     SpShared& s = sp_shared();
-    if (m.op == SP_FIRST) first_pass(m);
+    if (m.op == SP_FIRST) {
+      const bool with_k = m.high[SP_K] > -INFINITY, with_m = m.theta > -FLT_MAX;
+      if (with_k) with_m ? first_pass<true, true>(m) : first_pass<true, false>(m);
+      else with_m ? first_pass<false, true>(m) : first_pass<false, false>(m);
+    }
     if (m.op == SP_PASS) pass(m);
     if (m.op == SP_HIST) {
       s.hist4[threadIdx.x] = make_uint4(0, 0, 0, 0);

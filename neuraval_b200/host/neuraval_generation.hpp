@@ -283,6 +283,66 @@ class LogitsProcessor {
   Device& d_;
 };
 
+// The LM head with each request's low-rank adapter (ncb_adapter_head_*): what
+// ModernDecoderModel.ComputeLogits (ModernDecoderModel.cs:221-240) does for one
+// request, for the rows of many. dtype: NCB_DTYPE_F16 or NCB_DTYPE_BF16; all
+// pointers are device pointers, everything is ordered on the given stream.
+class AdapterHead {
+ public:
+  AdapterHead(int device, int dtype, int inFeatures, int outFeatures, int maxRows, int maxAdapters = 0,
+              int maxRank = 0)
+      : device_(device), in_(inFeatures), out_(outFeatures), max_rows_(maxRows) {
+    check(ncb_adapter_head_create(device, dtype, inFeatures, outFeatures, maxRows, maxAdapters,
+                                  maxRank, &h_),
+          "ncb_adapter_head_create");
+  }
+  ~AdapterHead() {
+    if (h_) ncb_adapter_head_destroy(h_);
+  }
+  AdapterHead(const AdapterHead&) = delete;
+  AdapterHead& operator=(const AdapterHead&) = delete;
+  int DeviceId() const { return device_; }
+  int InFeatures() const { return in_; }
+  int OutFeatures() const { return out_; }
+  int MaxRows() const { return max_rows_; }
+
+  // [outFeatures, inFeatures], rows ld apart; stays the caller's and in use.
+  void SetWeight(const void* weight, int64_t ld, cudaStream_t stream) const {
+    check(ncb_adapter_head_set_weight_device(h_, weight, ld, stream),
+          "ncb_adapter_head_set_weight_device");
+  }
+  // a [rank, inFeatures] and b [outFeatures, rank] are copied.
+  void SetAdapter(int slot, const void* a, int64_t lda, const void* b, int64_t ldb, int rank,
+                  float scale, cudaStream_t stream) const {
+    check(ncb_adapter_head_set_adapter_device(h_, slot, a, lda, b, ldb, rank, scale, stream),
+          "ncb_adapter_head_set_adapter_device");
+  }
+  void ClearAdapter(int slot, cudaStream_t stream) const {
+    check(ncb_adapter_head_clear_adapter_device(h_, slot, stream),
+          "ncb_adapter_head_clear_adapter_device");
+  }
+  // out [rows, outFeatures] of outDtype from x [rows, inFeatures]; adapterIds: a slot
+  // per row (-1: none), or nullptr.
+  void Project(const void* x, int64_t ldx, int rows, const int32_t* adapterIds, void* out,
+               int outDtype, int64_t ldo, cudaStream_t stream) const {
+    check(ncb_adapter_head_project_device(h_, x, ldx, rows, adapterIds, out, outDtype, ldo, stream),
+          "ncb_adapter_head_project_device");
+  }
+
+ private:
+  NcbAdapterHead* h_ = nullptr;
+  int device_, in_, out_, max_rows_;
+};
+
+// One request of TextGenerator::GenerateBatch: the reference's prompt and options,
+// and two settings it does not have, a min-p and the adapter slot of the head.
+struct BatchRequest {
+  std::vector<int> PromptTokenIds;
+  GenerationOptions Options;
+  float MinP = 0.0f;
+  int Adapter = -1;
+};
+
 // GenerationFinishReason (GenerationFinishReason.cs) and GenerationResult
 // (GenerationResult.cs:7-27).
 enum class GenerationFinishReason { MaxNewTokens, StopToken };
@@ -397,7 +457,117 @@ class TextGenerator {
     return result;
   }
 
+  // The last hidden states of the given contexts, [contexts, in_features] of the
+  // head's type in device memory, complete in stream order on `stream`.
+  using HiddenModel = std::function<const void*(const std::vector<std::vector<int>>& contexts,
+                                                cudaStream_t stream)>;
+
+  // Generate for many requests in step, each with options, random source and
+  // adapter of its own: per step the model's hidden states of the requests still
+  // running, the head's projection with their adapters and one sampling call with
+  // their options; 24 bytes per request go to the device and 4 come back.
+  // `randoms`: a source per request, or empty (each request then seeds its own).
+  // A request's tokens do not depend on the others'. Repetition, frequency and
+  // presence penalties are one value per call in the library, so a request that
+  // sets one is refused.
+  std::vector<GenerationResult> GenerateBatch(const HiddenModel& model, const AdapterHead& head,
+                                              const std::vector<BatchRequest>& requests,
+                                              cudaStream_t stream,
+                                              const std::vector<Random*>& randoms = {}) const {
+    if (!model) throw ArgumentNullException("model");
+    if (requests.empty()) return {};
+    if (static_cast<int>(requests.size()) > head.MaxRows()) throw ArgumentOutOfRangeException("requests");
+    if (!randoms.empty() && randoms.size() != requests.size()) throw ArgumentException("randoms");
+    for (const BatchRequest& r : requests) {
+      if (r.PromptTokenIds.empty()) throw ArgumentException("promptTokenIds");
+      if (!(r.MinP >= 0.0f && r.MinP <= 1.0f)) throw ArgumentOutOfRangeException("minP");
+      if (r.Options.RepetitionPenalty() != 1.0f || r.Options.FrequencyPenalty() != 0.0f ||
+          r.Options.PresencePenalty() != 0.0f)
+        throw ArgumentException("options");
+    }
+    const size_t n = requests.size(), vocab = static_cast<size_t>(head.OutFeatures());
+    int before = 0;
+    cuda(cudaGetDevice(&before), "cudaGetDevice");
+    cuda(cudaSetDevice(head.DeviceId()), "cudaSetDevice");
+    const auto restore = [before](void*) { cudaSetDevice(before); };
+    std::unique_ptr<void, decltype(restore)> device(this_address(), restore);
+    auto dev_free = [](void* p) { cudaFree(p); };
+    auto host_free = [](void* p) { cudaFreeHost(p); };
+    // per request: adapter, T, top_k, top_p, min_p, u; then the token
+    void* p = nullptr;
+    cuda(cudaMalloc(&p, 7 * 4 * n), "cudaMalloc");
+    std::unique_ptr<void, decltype(dev_free)> dmem(p, dev_free);
+    p = nullptr;
+    cuda(cudaMalloc(&p, sizeof(float) * n * vocab), "cudaMalloc");
+    std::unique_ptr<void, decltype(dev_free)> logits(p, dev_free);
+    p = nullptr;
+    cuda(cudaMallocHost(&p, 7 * 4 * n), "cudaMallocHost");
+    std::unique_ptr<void, decltype(host_free)> hmem(p, host_free);
+    int32_t* d = static_cast<int32_t*>(dmem.get());
+    int32_t* h = static_cast<int32_t*>(hmem.get());
+    std::vector<std::optional<DefaultRandom>> own(n);
+    std::vector<Random*> random(n);
+    for (size_t i = 0; i < n; ++i)
+      random[i] = randoms.empty() || !randoms[i] ? &own[i].emplace(SeedOf(requests[i].Options)) : randoms[i];
+    std::vector<std::vector<int>> sequences(n);
+    std::vector<GenerationResult> results(n);
+    std::vector<size_t> running;
+    for (size_t i = 0; i < n; ++i) {
+      sequences[i] = requests[i].PromptTokenIds;
+      if (requests[i].Options.MaxNewTokens() > 0) running.push_back(i);
+    }
+    while (!running.empty()) {
+      const size_t rows = running.size();
+      std::vector<std::vector<int>> contexts;
+      for (size_t i : running) contexts.push_back(Trim(sequences[i]));
+      const void* hidden = model(contexts, stream);
+      if (!hidden) throw ArgumentNullException("hidden");
+      for (size_t j = 0; j < rows; ++j) {
+        const BatchRequest& r = requests[running[j]];
+        const bool greedy = r.Options.Greedy();
+        const float T = greedy ? 0.0f : r.Options.Temperature(), top_p = r.Options.TopP(),
+                    u = greedy ? 0.0f : static_cast<float>(random[running[j]]->NextDouble());
+        h[j] = r.Adapter;
+        std::memcpy(h + rows + j, &T, 4);
+        h[2 * rows + j] = r.Options.TopK();
+        std::memcpy(h + 3 * rows + j, &top_p, 4);
+        std::memcpy(h + 4 * rows + j, &r.MinP, 4);
+        std::memcpy(h + 5 * rows + j, &u, 4);
+      }
+      cuda(cudaMemcpyAsync(d, h, 6 * 4 * rows, cudaMemcpyHostToDevice, stream), "cudaMemcpyAsync");
+      head.Project(hidden, head.InFeatures(), static_cast<int>(rows), d, logits.get(), NCB_DTYPE_F32,
+                   static_cast<int64_t>(vocab), stream);
+      const float* f = reinterpret_cast<const float*>(d);
+      check(ncb_sample_rows_min_p_device(logits.get(), NCB_DTYPE_F32, static_cast<int>(rows),
+                                         static_cast<int>(vocab), static_cast<int64_t>(vocab),
+                                         f + 5 * rows, f + rows, d + 2 * rows, f + 3 * rows,
+                                         f + 4 * rows, d + 6 * rows, nullptr, nullptr, nullptr, stream),
+            "ncb_sample_rows_min_p_device");
+      cuda(cudaMemcpyAsync(h + 6 * rows, d + 6 * rows, 4 * rows, cudaMemcpyDeviceToHost, stream),
+           "cudaMemcpyAsync");
+      cuda(cudaStreamSynchronize(stream), "cudaStreamSynchronize");
+      std::vector<size_t> still;
+      for (size_t j = 0; j < rows; ++j) {
+        const size_t i = running[j];
+        const int next = h[6 * rows + j];
+        if (next < 0) throw CudaException(NCB_ERROR_INVALID_ARGUMENT, "GenerateBatch: row not sampled");
+        results[i].GeneratedTokenIds.push_back(next);
+        sequences[i].push_back(next);
+        if (IsStop(requests[i].Options, next))
+          results[i].FinishReason = GenerationFinishReason::StopToken;
+        else if (static_cast<int>(results[i].GeneratedTokenIds.size()) < requests[i].Options.MaxNewTokens())
+          still.push_back(i);
+      }
+      running.swap(still);
+    }
+    return results;
+  }
+
  private:
+  static void* this_address() {  // anything but null: a unique_ptr calls its deleter for it
+    static char c;
+    return &c;
+  }
   static uint64_t SeedOf(const GenerationOptions& o) {
     return o.Seed() ? static_cast<uint64_t>(*o.Seed()) : std::random_device{}();
   }

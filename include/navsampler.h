@@ -372,10 +372,13 @@ NCB_API int ncb_sample_rows_min_p_device(const void* d_logits, int dtype, int ro
  *   out[n, :] = W x_n + scale_s * B_s (A_s x_n),  s = adapter_ids[n]
  * W is [out_features, in_features], A_s [rank_s, in_features], B_s
  * [out_features, rank_s], x [rows, in_features], all of the handle's dtype
- * (NCB_DTYPE_F16 or NCB_DTYPE_BF16). Products are summed in fp32 (A_s x_n too)
- * and rounded once, to the output's type. No sum's order depends on timing: the
- * same call gives the same bits, and a row's values depend on no other row's
- * x or adapter.
+ * (NCB_DTYPE_F16 or NCB_DTYPE_BF16). Products are summed in fp32 and rounded
+ * once, to the output's type; scale_s A_s x_n goes into the second product as the
+ * sum of two values of the handle's type (2^-16 of it or less is lost). No sum's
+ * order depends on timing: the same call gives the same bits. A row whose adapter
+ * holds a NaN or an infinity, or whose scale_s A_s x_n is not finite in the
+ * handle's type (fp16: beyond 65504), comes back as NaN; no other row of the call
+ * is touched by it.
  *
  * The handle owns packed copies of the adapters and its scratch; like a
  * sampler it is single-stream: calls on one handle must not overlap on the GPU
@@ -389,7 +392,9 @@ typedef struct NcbAdapterHead NcbAdapterHead;
 NCB_API int ncb_adapter_head_create(int device, int dtype, int in_features, int out_features,
                                     int max_rows, int max_adapters, int max_rank,
                                     NcbAdapterHead** out);
-/* Waits for the device before it frees. */
+/* Waits for the device before it frees. Returns NCB_ERROR_LAUNCH_FAILED (and frees)
+ * if a wait inside one of the handle's kernels ever gave up after its 2 s, which
+ * leaves that call's output undefined. */
 NCB_API int ncb_adapter_head_destroy(NcbAdapterHead* head);
 /* The shared weight, rows `ld` elements apart. It is read in place by later
  * calls and has to stay allocated, except where its base or row stride is not a

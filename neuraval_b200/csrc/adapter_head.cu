@@ -49,7 +49,7 @@ constexpr int AH_MAX_STAGES = 12;
 constexpr int AH_SMEM = 208 * 1024;  // stages; leaves room for a shrink CTA on the SM
 constexpr int AH_EPILOGUE = 8;    // warps that write results
 constexpr int AH_THREADS = (AH_EPILOGUE + 2) * 32;  // and a copying and a multiplying one
-constexpr int AH_PIECE = 8;       // stages added up in TMEM for an fp32 output
+constexpr int AH_PIECE = 4;       // stages added up in TMEM for an fp32 output
 constexpr int AH_SINGLE = 64;     // rows per tile up to which single CTAs work, unsorted
 constexpr int AH_BLOCK = 32;      // rows per block of larger tiles
 __host__ __device__ constexpr int ah_per(int group) { return group == 1 ? 2 : 4; }  // adapter entries per stage
@@ -366,9 +366,9 @@ __global__ void __launch_bounds__(AU_THREADS, 4) adapter_shrink_kernel(const AhA
 #pragma unroll
     for (int w = 0; w < AU_THREADS / 32; ++w) v += part[w][t];
     v *= g.scales[slot];
-    if (g.ranks[slot] < 0) v = NAN;
-    const E hi = E(v);
-    const E lo = E(fabsf((float)hi) < INFINITY ? v - (float)hi : 0.0f);
+    E hi = E(v);
+    if (g.ranks[slot] < 0 || !(fabsf((float)hi) < INFINITY)) hi = E(NAN);
+    const E lo = E(v - (float)hi);
     E* to = row_of(own + slice * next, place) + ah_at(place % g.bh, t);
     to[0] = hi;
     to[(int64_t)g.bh * 16] = lo;
@@ -1041,14 +1041,16 @@ NCB_API int ncb_adapter_head_create(int device, int dtype, int in_features, int 
 
 NCB_API int ncb_adapter_head_destroy(NcbAdapterHead* h) {
   if (!h) return ncb_record_status(NCB_ERROR_INVALID_ARGUMENT);
+  uint32_t error = 0;
   {
     AhDevice guard(h->device);
     cudaDeviceSynchronize();
+    if (cudaMemcpy(&error, h->error_word, sizeof(error), cudaMemcpyDeviceToHost) != cudaSuccess) error = 1;
     cudaFree(h->mem);
     cudaFree(h->w_own);
   }
   delete h;
-  return ncb_record_status(NCB_OK);
+  return ncb_record_status(error ? NCB_ERROR_LAUNCH_FAILED : NCB_OK);
 }
 
 NCB_API int ncb_adapter_head_set_weight_device(NcbAdapterHead* h, const void* d_weight, int64_t ld,

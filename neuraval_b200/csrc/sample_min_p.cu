@@ -79,7 +79,7 @@ struct SpArgs {
   uint32_t* flags;
 };
 
-enum { SP_DONE, SP_FIRST, SP_PASS, SP_HIST, SP_GATHER, SP_SELECT };
+enum { SP_DONE, SP_FIRST, SP_PASS, SP_HIST, SP_GATHER, SP_STREAM, SP_SELECT };
 enum { SP_K = 0, SP_P = 1, SP_D = 2, SP_WINDOWS = 3 };
 
 struct SpCmd {
@@ -194,6 +194,15 @@ struct SpVec<__half> {
   static __device__ __forceinline__ uint32_t none() { return 0xFC00u; }
 };
 
+// The row passes by the L1 cache: what does not fit into registers lives there.
+__device__ __forceinline__ uint4 sp_load(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
 // A CTA's slice: 16-byte granules [g0, g0 + n) of the row, granule 0 starting at
 // the 16-byte boundary at or below the row's first value. Only the row's first and
 // last granule can hold values of other rows; they are read value by value and
@@ -235,39 +244,55 @@ struct SpSlice {
   // f(values, granule) for this thread's granules, FLIGHT loads at a time. The whole
   // granules are read without a branch (the loads would wait for one another); past
   // the end the last one is read again and dropped.
+  // Granules [begin, end) of the slice.
   template <int FLIGHT, int THREADS, typename F>
-  __device__ __forceinline__ void each_granule(F f) const {
+  __device__ __forceinline__ void each_granule(F f, int begin, int end) const {
     constexpr int N = SpVec<E>::N;
-    const int lo = n > 0 && g0 * N < skip ? 1 : 0;
-    const int hi = n > lo && (g0 + n) * N - skip > vocab ? n - 1 : n;
+    const bool front = begin == 0 && end > 0 && g0 * N < skip,
+               back = end == n && end > begin + (front ? 1 : 0) && (g0 + n) * N - skip > vocab;
+    const int lo = begin + (front ? 1 : 0), hi = end - (back ? 1 : 0);
     const uint4* from = reinterpret_cast<const uint4*>(base) + g0;
     uint4 g[FLIGHT];
     auto load = [&](int i0) {
 #pragma unroll
-      for (int j = 0; j < FLIGHT; ++j) g[j] = __ldg(from + min(i0 + j * THREADS, hi - 1));
+      for (int j = 0; j < FLIGHT; ++j) g[j] = sp_load(from + min(i0 + j * THREADS, hi - 1));
     };
     const int i0 = lo + threadIdx.x;
-    if (lo < hi) load(i0);
+    if constexpr (FLIGHT < 4) {
+      if (lo < hi) load(i0);
 #pragma unroll 1
-    for (int i = i0; i < hi; i += FLIGHT * THREADS) {
-      uint4 now[FLIGHT];
+      for (int i = i0; i < hi; i += FLIGHT * THREADS) {
+        uint4 now[FLIGHT];
 #pragma unroll
-      for (int j = 0; j < FLIGHT; ++j) now[j] = g[j];
-      load(i + FLIGHT * THREADS);  // on its way while f works
+        for (int j = 0; j < FLIGHT; ++j) now[j] = g[j];
+        load(i + FLIGHT * THREADS);  // on its way while f works
 #pragma unroll
-      for (int j = 0; j < FLIGHT; ++j)
-        if (i + j * THREADS < hi) f(now[j], i + j * THREADS);
+        for (int j = 0; j < FLIGHT; ++j)
+          if (i + j * THREADS < hi) f(now[j], i + j * THREADS);
+      }
+    } else {  // light work: the other warps' loads are on their way
+#pragma unroll 1
+      for (int i = i0; i < hi; i += FLIGHT * THREADS) {
+        load(i);
+#pragma unroll
+        for (int j = 0; j < FLIGHT; ++j)
+          if (i + j * THREADS < hi) f(g[j], i + j * THREADS);
+      }
     }
-    const int edge = threadIdx.x == 0 && lo ? 0 : threadIdx.x == 32 && hi < n ? n - 1 : -1;
+    const int edge = threadIdx.x == 0 && front ? 0 : threadIdx.x == 32 && back ? n - 1 : -1;
     if (edge >= 0) f(fetch(edge), edge);
   }
   template <int FLIGHT, typename F>
-  __device__ __forceinline__ void each(F f) const {
+  __device__ __forceinline__ void each(F f, int begin, int end) const {
     each_granule<FLIGHT, SP_NT>([&](const uint4& g, int i) {
       float v[SpVec<E>::N];
       SpVec<E>::get(g, v);
       f(v, i);
-    });
+    }, begin, end);
+  }
+  template <int FLIGHT, typename F>
+  __device__ __forceinline__ void each(F f) const {
+    each<FLIGHT>(f, 0, n);
   }
   // Of the row at x, the part of CTA `rank`: `per` granules.
   __device__ __forceinline__ void set(const E* x, int vocab_, int rank, int per) {
@@ -446,12 +471,72 @@ struct SpRow {
   SpSlice<E> sl;
   cg::cluster_group cl;
   int rank, ranks;
+  float T;
+  int part;  // granules of the slice that the first pass looks at
   SpView k;
+
+  // Greatest and least finite value of the CTA's threads to every CTA of the row.
+  __device__ void share(float mx, float mn) {
+    SpShared& s = sp_shared();
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      mx = sp_max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+    }
+    if ((threadIdx.x & 31) == 0) {
+      s.red_f[threadIdx.x >> 5] = mx;
+      s.red_i[threadIdx.x >> 5] = __float_as_int(mn);
+    }
+    __syncthreads();
+    if (threadIdx.x < ranks) {
+      for (int w = 0; w < SP_NT / 32; ++w) {
+        mx = sp_max_nan(mx, s.red_f[w]);
+        mn = fminf(mn, __int_as_float(s.red_i[w]));
+      }
+      of(threadIdx.x).mx[rank] = mx;
+      of(threadIdx.x).mn[rank] = mn;
+    }
+  }
+  // From what all have shared: the maximum, and what values mean below it.
+  __device__ float view() {
+    SpShared& s = sp_shared();
+    float mx = s.mx[0], mn = s.mn[0];
+    for (int r = 1; r < ranks; ++r) {
+      mx = sp_max_nan(mx, s.mx[r]);
+      mn = fminf(mn, s.mn[r]);
+    }
+    k.mx = mx;
+    k.inv_t = 1.0 / (double)T;
+    k.c = k.inv_t / 0.69314718055994530942;
+    // bins over the finite values, as far as they carry mass
+    const double far = (double)mx - SP_REACH * (double)T;
+    k.zero = far > -(double)FLT_MAX ? (float)far : -FLT_MAX;
+    k.scale = (float)fmin((SP_BINS - 1) / ((double)mx - fmax((double)mn, far)), (double)FLT_MAX);
+    return mx;
+  }
+  static __device__ __forceinline__ bool finite(float x) { return x >= -FLT_MAX && x <= FLT_MAX; }
+  template <bool LIST>
+  static __device__ __forceinline__ void take(const SpSlice<E>& sl, const float* v, int i, float least,
+                                              float& mx, float& mn) {
+    float most = v[0];
+#pragma unroll
+    for (int e = 0; e < SpVec<E>::N; ++e) {
+      if (e) most = sp_max_nan(most, v[e]);
+      mn = fminf(mn, v[e] == -INFINITY ? INFINITY : v[e]);
+    }
+    mx = sp_max_nan(mx, most);
+    if (LIST && !(most < least)) {  // (or a NaN, which hides the others; the row is bad then)
+#pragma unroll
+      for (int e = 0; e < SpVec<E>::N; ++e)
+        if (v[e] >= least) put(0, 0, SP_FEW, v[e], sl.id(i, e));
+    }
+  }
 
   __device__ __forceinline__ SpShared& of(int r) { return *cl.map_shared_rank(&sp_shared(), r); }
 
   // ---- the commands, carried out by every CTA of the cluster ------------------
   __device__ __noinline__ void hist_by_value() {
+    const SpSlice<E> sl = this->sl;
     SpShared& s = sp_shared();
     const SpView k = this->k;
     sl.template each<2>([&](const float* v, int) {
@@ -465,6 +550,7 @@ struct SpRow {
     });
   }
   __device__ __noinline__ void hist_by_key(const SpCmd& m) {
+    const SpSlice<E> sl = this->sl;
     SpShared& s = sp_shared();
     sl.template each<1>([&](const float* v, int) {
 #pragma unroll
@@ -477,26 +563,48 @@ struct SpRow {
       }
     });
   }
-  __device__ __forceinline__ void put(SpShared& to, int w, int base, int cap, float v, int id) {
+  // A value into the CTA's own list w (places [base, base + cap) of `list`). CTA 0's is
+  // the row's; the others hand theirs over after a pass (an atomic on another CTA's
+  // memory holds a warp up for a microsecond; a call that is not inlined, three).
+  static __device__ __forceinline__ void put(int w, int base, int cap, float v, int id) {
     SpShared& s = sp_shared();
-    const int at = atomicAdd(&to.n_list[w], 1);
+    const int at = atomicAdd(&s.n_list[w], 1);
     if (at < cap)
-      to.list[base + at] = ((unsigned long long)sp_key(v) << 32) | (0xFFFFFFFFu - (uint32_t)id);
+      s.list[base + at] = ((unsigned long long)sp_key(v) << 32) | (0xFFFFFFFFu - (uint32_t)id);
   }
-  __device__ __noinline__ void gather(const SpCmd& m) {
+  __device__ void hand_over(int w, int base, int cap) {
+    if (rank == 0) return;
     SpShared& s = sp_shared();
     SpShared& to = of(0);
+    __syncthreads();
+    const int n = s.n_list[w];
+    if (n == 0) return;
+    if (threadIdx.x == 0) s.got_i = atomicAdd(&to.n_list[w], n);
+    __syncthreads();
+    const int at = s.got_i;
+    for (int i = threadIdx.x; i < min(n, cap); i += SP_NT)
+      if (at + i < cap) to.list[base + at + i] = s.list[base + i];
+    __syncthreads();
+    if (threadIdx.x == 0) s.n_list[w] = 0;
+  }
+  __device__ __noinline__ void gather(const SpCmd& m) {
+    const SpSlice<E> sl = this->sl;
     const float least = m.theta;
-    sl.template each<4>([&](const float* v, int i) {
-      float most = v[0];
-#pragma unroll
-      for (int e = 1; e < SpVec<E>::N; ++e) most = fmaxf(most, v[e]);
-      if (most >= least) {
-#pragma unroll
-        for (int e = 0; e < SpVec<E>::N; ++e)
-          if (v[e] >= least) put(to, 0, 0, SP_FEW, v[e], sl.id(i, e));
-      }
-    });
+    float mx = -INFINITY, mn = INFINITY;
+    sl.template each<4>([&](const float* v, int i) { take<true>(sl, v, i, least, mx, mn); });
+    hand_over(0, 0, SP_FEW);
+  }
+  // What the first pass left, with its maximum, and the values from `theta` on of all.
+  __device__ __noinline__ void stream(const SpCmd& m) {
+    const SpSlice<E> sl = this->sl;
+    SpShared& s = sp_shared();
+    const float least = m.theta;
+    float mx = s.mx[rank], mn = s.mn[rank];
+    sl.template each<4>([&](const float* v, int i) { take<true>(sl, v, i, least, mx, mn); }, part, sl.n);
+    sl.template each<4>([&](const float* v, int i) { take<true>(sl, v, i, least, mx, mn); }, 0, part);
+    hand_over(0, 0, SP_FEW);
+    __syncthreads();
+    share(mx, mn);
   }
   // The usual pass: windows that are runs of bins. Exact masses above each and of what
   // min-p keeps; the values of a window into its list, or, where they are too many,
@@ -504,6 +612,7 @@ struct SpRow {
   // WITH_K: K's mass ends at a window too (otherwise it is the row's); WITH_M: min-p is on.
   template <bool WITH_K, bool WITH_M>
   __device__ __noinline__ void first_pass(const SpCmd& m) {
+    const SpSlice<E> sl = this->sl;
     SpShared& s = sp_shared();
     const SpView k = this->k;
     SpShared& to = of(0);
@@ -557,7 +666,7 @@ struct SpRow {
           for (int w = 0; w < SP_WINDOWS; ++w)
             if (x <= hi[w] && x >= lo[w]) {
               if (m.gather[w]) {
-                put(to, w, w * SP_CAP, SP_CAP, x, sl.id(i, e));
+                put(w, w * SP_CAP, SP_CAP, x, sl.id(i, e));
               } else {
                 low[w] = min(low[w], sp_key(x));
                 high[w] = max(high[w], sp_key(x));
@@ -566,6 +675,8 @@ struct SpRow {
         }
       }
     });
+    for (int w = 0; w < SP_WINDOWS; ++w)
+      if (m.gather[w]) hand_over(w, w * SP_CAP, SP_CAP);
 #pragma unroll
     for (int j = 0; j <= SP_WINDOWS; ++j)
 #pragma unroll
@@ -610,6 +721,7 @@ struct SpRow {
   }
   // Any windows, by their keys, with what lies in them; those that fit are listed.
   __device__ __noinline__ void pass(const SpCmd& m) {
+    const SpSlice<E> sl = this->sl;
     SpShared& s = sp_shared();
     const SpView k = this->k;
     SpShared& to = of(0);
@@ -634,7 +746,7 @@ struct SpRow {
           } else if (x >= lo[w]) {
             p.mass[SP_WINDOWS + 1 + w] += wt;
             ++p.n[SP_WINDOWS + 1 + w];
-            if (m.gather[w]) put(to, w, w * SP_CAP, SP_CAP, x, sl.id(i, e));
+            if (m.gather[w]) put(w, w * SP_CAP, SP_CAP, x, sl.id(i, e));
           }
         }
         if (x >= m.theta) {
@@ -643,6 +755,8 @@ struct SpRow {
         }
       }
     });
+    for (int w = 0; w < SP_WINDOWS; ++w)
+      if (m.gather[w]) hand_over(w, w * SP_CAP, SP_CAP);
 #pragma unroll
     for (int j = 0; j < SP_SUMS; ++j) {
 #pragma unroll
@@ -666,6 +780,7 @@ struct SpRow {
   // The id of the nth occurrence of a value, counted over the CTAs in the order of
   // their slices and inside a CTA over its threads, each with granules in a row.
   __device__ __noinline__ void select(const SpCmd& m) {
+    const SpSlice<E> sl = this->sl;
     SpShared& s = sp_shared();
     const int q = (sl.n + SP_NT - 1) / SP_NT;
     const int b = min(sl.n, (int)threadIdx.x * q), e = min(sl.n, b + q);
@@ -707,6 +822,7 @@ struct SpRow {
       else hist_by_key(m);
     }
     if (m.op == SP_GATHER) gather(m);
+    if (m.op == SP_STREAM) stream(m);
     if (m.op == SP_SELECT) select(m);
   }
   // CTA 0: s.cmd to every CTA, carried out by all; returns when all are done.
@@ -722,6 +838,7 @@ struct SpRow {
     const SpCmd m = s.cmd;
     carry_out(m);
     cl.sync();
+    if (m.op == SP_STREAM) view();
   }
   __device__ void obey() {
     SpShared& s = sp_shared();
@@ -731,6 +848,7 @@ struct SpRow {
       if (m.op == SP_DONE) return;
       carry_out(m);
       cl.sync();
+      if (m.op == SP_STREAM) view();
     }
   }
 
@@ -925,7 +1043,6 @@ struct SpWindow {
 template <typename E>
 __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) {
   SpShared& s = sp_shared();
-  constexpr int N = SpVec<E>::N;
   SpRow<E> R{{}, cg::this_cluster()};
   R.rank = (int)R.cl.block_rank();
   R.ranks = (int)R.cl.num_blocks();
@@ -943,71 +1060,51 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
   const bool greedy = T == 0.0f;
 
   R.cl.barrier_arrive();  // this CTA runs: the others may write into it
-  // ---- load, maximum, least finite value ---------------------------------------------
   R.sl.set(static_cast<const E*>(a.logits) + (int64_t)row * a.ld, a.vocab, R.rank, a.per);
+  R.T = T;
   s.hist4[t] = make_uint4(0, 0, 0, 0);
   if (t < SP_WINDOWS) s.n_list[t] = 0;
+  // ---- maximum, least finite value; where few values are wanted, of a part of the row first --------
+  const bool bounded = !greedy && k_asked > 0 && k_asked <= min(SP_BOUNDED, SP_NT * R.ranks / 2);
+  bool few = bounded || (!greedy && min_p > 0.0f && top_p >= 1.0f);
+  R.part = R.sl.n;
+  // (of short slices all: reading them again costs less than sorting more)
+  if (few && R.sl.n > 4 * SP_NT)
+    R.part = ((k_asked > SP_BOUNDED / 2 ? R.sl.n / 2 : R.sl.n / 4) + SP_NT - 1) / SP_NT * SP_NT;
   float mx = -INFINITY, mn = INFINITY;
-  R.sl.template each<4>([&](const float* v, int) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      mx = sp_max_nan(mx, v[e]);
-      mn = fminf(mn, v[e] == -INFINITY ? INFINITY : v[e]);
-    }
-  });
-  const float own = mx;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    mx = sp_max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-  }
-  if ((t & 31) == 0) {
-    s.red_f[t >> 5] = mx;
-    s.red_d[t >> 5] = mn;
-  }
-  __syncthreads();
+  R.sl.template each<4>([&](const float* v, int i) { SpRow<E>::template take<false>(R.sl, v, i, 0.0f, mx, mn); }, 0, R.part);
+  float own = mx;
   R.cl.barrier_wait();
-  if (t < R.ranks) {
-    for (int w = 0; w < SP_NT / 32; ++w) {
-      mx = sp_max_nan(mx, s.red_f[w]);
-      mn = fminf(mn, (float)s.red_d[w]);
-    }
-    R.of(t).mx[R.rank] = mx;
-    R.of(t).mn[R.rank] = mn;
-  }
+  R.share(mx, mn);
   R.cl.sync();
-  mx = s.mx[0];
-  mn = s.mn[0];
-  for (int r = 1; r < R.ranks; ++r) {
-    mx = sp_max_nan(mx, s.mx[r]);
-    mn = fminf(mn, s.mn[r]);
+  float top = R.view();
+  if (few && top == -INFINITY) {  // nothing there: as if many were wanted
+    few = false;
+    R.cl.sync();
+    R.sl.template each<4>([&](const float* v, int i) { SpRow<E>::template take<false>(R.sl, v, i, 0.0f, mx, mn); }, R.part, R.sl.n);
+    R.share(mx, mn);
+    R.cl.sync();
+    top = R.view();
   }
-  if (!(mx >= -FLT_MAX && mx <= FLT_MAX)) {
+  if (!R.finite(top)) {
     if (R.rank == 0 && t == 0) sp_write_bad(a, row, NCB_FLAG_NONFINITE);
     return;
   }
-  R.k.mx = mx;
   if (greedy) {
     SpCmd m{};
     m.op = SP_SELECT;
-    m.value = mx;
+    m.value = top;
     R.select(m);
     R.cl.sync();
     if (R.rank == 0 && t == 0) sp_write(a, row, s.token, 0.0f, 1, 0);
     return;
   }
-  R.k.inv_t = 1.0 / (double)T;
-  R.k.c = R.k.inv_t / 0.69314718055994530942;
-  // bins over the finite values, as far as they carry mass
-  const double far = (double)mx - SP_REACH * (double)T;
-  R.k.zero = far > -(double)FLT_MAX ? (float)far : -FLT_MAX;
-  R.k.scale = (float)fmin((SP_BINS - 1) / ((double)mx - fmax((double)mn, far)), (double)FLT_MAX);
 
   // ---- few values wanted: those above a bound ------------------------------------------
   // The threads' maxima are so many different values of the row: the bin of the k-th
-  // largest of them, or an earlier one, holds the k-th value.
-  const bool bounded = k_asked > 0 && k_asked <= min(SP_BOUNDED, SP_NT * R.ranks / 2);
-  const bool few = bounded || (min_p > 0.0f && top_p >= 1.0f);
+  // largest of them, or an earlier one, holds the k-th value. The bound comes from the
+  // first quarter or half of the row (of which about four or two times k values are
+  // above it in the whole row), so that the rest is read once.
   if (few) {
     if (bounded && own > -INFINITY) atomicAdd(reinterpret_cast<int*>(s.hist4) + R.k.bin(own), 1);
     R.cl.sync();
@@ -1019,29 +1116,38 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
     R.obey();
     return;
   }
-  if (t == 0) s.theta = sp_least_kept(mx, T, min_p, R.k.inv_t);
-  const float step = (float)(R.k.inv_t / (double)R.k.scale);  // nats per bin
+  float step;  // nats per bin
   auto centre = [&](int b) { return __expf(-((float)b + 0.5f) * step); };
   if (few) {
-    int deep = SP_BINS - 1;  // the last bin that has to be known
+    step = 0.0f;
+    float least = -FLT_MAX;
     if (bounded) {
       const int maxima = R.merge(centre, false);
-      if (maxima >= k_asked) deep = R.bin_of_count(k_asked, maxima);
+      if (maxima >= k_asked) {
+        const int deep = R.bin_of_count(k_asked, maxima);
+        // not above any value of these bins, whose places are off by 2^-23 of them at most
+        const double edge = (double)top - (deep + 1) / (double)R.k.scale * (1.0 + 1e-6);
+        if (deep < SP_BINS - 1 && edge > -(double)FLT_MAX) least = nextafterf((float)edge, -INFINITY);
+      }
     }
+    // the part's maximum is not above the row's, and so is what min-p keeps
+    if (t == 0) s.theta = top_p >= 1.0f ? fmaxf(least, sp_least_kept(top, T, min_p, R.k.inv_t)) : least;
     __syncthreads();
-    if (min_p > 0.0f && top_p >= 1.0f) deep = min(deep, R.k.bin(s.theta));
     if (t == 0) {
-      s.cmd.op = SP_GATHER;
-      // not above any value of these bins, whose places are off by 2^-23 of them at most
-      const double edge = (double)mx - (deep + 1) / (double)R.k.scale * (1.0 + 1e-6);
-      s.cmd.theta = deep == SP_BINS - 1 || !(edge > -(double)FLT_MAX) ? -FLT_MAX
-                                                                     : nextafterf((float)edge, -INFINITY);
+      s.cmd.op = SP_STREAM;
+      s.cmd.theta = s.theta;
     }
     R.command();
+    top = R.k.mx;
+    if (t == 0) s.theta = sp_least_kept(top, T, min_p, R.k.inv_t);
     const int n = s.n_list[0];
-    if (n <= SP_FEW) {
+    if (!R.finite(top) || n <= SP_FEW) {
       if (t == 0) s.cmd.op = SP_DONE;
       R.command();
+      if (!R.finite(top)) {
+        if (t == 0) sp_write_bad(a, row, NCB_FLAG_NONFINITE);
+        return;
+      }
       sp_sort(s.list, n);
       const int k = k_asked > 0 ? k_asked : n;  // (fewer finite values than k: all of them are here)
       if (n <= SP_NT) R.template decide<1>(a, row, n, k, top_p, s.theta, u);
@@ -1053,7 +1159,11 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
       s.cmd.shift = -1;
     }
     R.command();
+  } else if (t == 0) {
+    s.theta = sp_least_kept(top, T, min_p, R.k.inv_t);
   }
+  mx = top;
+  step = (float)(R.k.inv_t / (double)R.k.scale);
   const int total = R.merge(centre, true);
   const int k = k_asked > 0 && k_asked < total ? k_asked : total;
   const int bk = R.bin_of_count(k, total);
@@ -1500,7 +1610,7 @@ __global__ void __launch_bounds__(SQ_NT, 1) sample_min_p16_kernel(const SpArgs a
         if (lo != none) atomicAdd(&counts[lo >> 1], 1u << ((lo & 1) * 16));
         if (hi != none) atomicAdd(&counts[hi >> 1], 1u << ((hi & 1) * 16));
       }
-    });
+    }, 0, sl.n);
   }
   R.cl.sync();
 
@@ -1738,7 +1848,7 @@ __global__ void __launch_bounds__(SQ_NT, 1) sample_min_p16_kernel(const SpArgs a
   sl.template each_granule<4, SQ_NT>([&](const uint4& g, int i) {
     const uint32_t yes = matches(g);
     if (yes) atomicAdd(&s.in_warp[i / SQ_NT][i % SQ_NT / 32], __popc(yes));
-  });
+  }, 0, sl.n);
   __syncthreads();
   int mine = 0;  // thread i < SQ_TILES * 32: part i
   if (t < SQ_TILES * 32) mine = s.in_warp[t / 32][t % 32];
@@ -1799,6 +1909,15 @@ int sp_start(void (*kernel)(nvs::SpArgs), nvs::SpArgs a, int rows, int granules,
   return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? NCB_OK : NCB_ERROR_LAUNCH_FAILED;
 }
 
+// A kernel's attribute, set once per device (twice is harmless).
+bool sp_once(std::atomic<int>* done, int device, int bit, void (*kernel)(nvs::SpArgs),
+             cudaFuncAttribute which, int value) {
+  if (device < SP_DEVICES && (done[device].load(std::memory_order_acquire) & bit)) return true;
+  if (cudaFuncSetAttribute(kernel, which, value) != cudaSuccess) return false;
+  if (device < SP_DEVICES) done[device].fetch_or(bit, std::memory_order_release);
+  return true;
+}
+
 template <typename E>
 int sp_launch(const nvs::SpArgs& a, int rows, int device, int num_sms, cudaStream_t st) {
   // Granules of a row, counting a first one that starts before it.
@@ -1818,12 +1937,9 @@ int sp_launch(const nvs::SpArgs& a, int rows, int device, int num_sms, cudaStrea
                           : ranks == 2 ? nvs::sample_min_p16_kernel<E, 2>
                           : ranks == 4 ? nvs::sample_min_p16_kernel<E, 4>
                                        : nvs::sample_min_p16_kernel<E, 8>;
-      static std::atomic<int> raised[SP_DEVICES];  // per device, a bit per kernel; twice is harmless
-      if (device >= SP_DEVICES || !(raised[device].load(std::memory_order_acquire) & ranks)) {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-          return NCB_ERROR_LAUNCH_FAILED;
-        if (device < SP_DEVICES) raised[device].fetch_or(ranks, std::memory_order_release);
-      }
+      static std::atomic<int> raised[SP_DEVICES];  // a bit per kernel
+      if (!sp_once(raised, device, ranks, kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))
+        return NCB_ERROR_LAUNCH_FAILED;
       return sp_start(kernel, a, rows, granules, ranks, nvs::SQ_NT, smem, st);
     }
   }
@@ -1833,6 +1949,10 @@ int sp_launch(const nvs::SpArgs& a, int rows, int device, int num_sms, cudaStrea
   while (ranks < nvs::SP_CLUSTER && (int64_t)rows * ranks * 2 <= 2 * num_sms &&
          granules / ranks >= 2 * nvs::SP_NT)
     ranks *= 2;
+  // two CTAs to an SM: without the request the SM was left split for one (89 -> 138 us)
+  static std::atomic<int> split[SP_DEVICES];
+  if (!sp_once(split, device, 1, nvs::sample_min_p_kernel<E>, cudaFuncAttributePreferredSharedMemoryCarveout, 40))
+    return NCB_ERROR_LAUNCH_FAILED;
   return sp_start(nvs::sample_min_p_kernel<E>, a, rows, granules, ranks, nvs::SP_NT,
                   sizeof(nvs::SpShared), st);
 }

@@ -7,7 +7,9 @@ random values, within a tolerance derived from the arithmetic:
     running sum (2^-23 where the hardware truncates, but then for 16 products at
     once); the running sum of products with random signs stays below 6 times
     their 2-norm q, so (K + R + 32) 2^-24 6 q covers them;
-  - A_s x_n, a sum of the same kind, multiplied with B_s;
+  - A_s x_n carried as the sum of two 16-bit values: off by 2^-16 relative
+    (bf16: two roundings of 2^-9 and more; fp16: more exact, down to its least
+    step, 2^-24), so 2^-16 |B_s| |u| + 2^-24 |B_s| 1;
   - the output's own rounding, half a step of its type.
 """
 import numpy as np
@@ -62,7 +64,7 @@ class Case:
                 q[n] += (b ** 2) @ (u ** 2)
                 # u itself, a sum in fp32
                 du = (self.inner + 32) * 2.0 ** -24 * 6 * self.scales[i] * ((a ** 2) @ (x[n] ** 2)).sqrt()
-                tol[n] += b.abs() @ (2.0 ** -23 * u.abs() + du)
+                tol[n] += b.abs() @ (2.0 ** -16 * u.abs() + 2.0 ** -24 + du)
         return y, tol + (self.inner + R + 32) * 2.0 ** -24 * 6 * q.sqrt()
 
     def head(self, max_rows=None, max_adapters=None, max_rank=None):
@@ -240,6 +242,19 @@ def test_non_finite_rows_stay_alone():
             assert not got[1::2].isfinite().all() and (got[::2] == want[::2]).all()
             h.set_adapter(1, c.a[0], c.b[0], 1.0)  # a sound one in its place
             assert c.run(h).isfinite().all()
+
+
+def test_overflowing_adapter_product_stays_in_its_row():
+    """fp16: scale A x beyond the type's range gives NaN in its row, and only there."""
+    import torch
+    c = Case(90, 64, 300, [8, 8], np.arange(90) % 2, "f16", 17, whole=True)
+    want = c.want()[0].float()
+    c.x[3] = 1000.0
+    c.a[1][:] = 10.0
+    with c.head() as h:
+        got = c.run(h)
+    assert got[3].isnan().all() and (got[::2] == want[::2]).all()
+    assert got[1::2][torch.arange(45) != 1].isfinite().all()
 
 
 def test_refusals_with_a_head():

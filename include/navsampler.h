@@ -374,8 +374,8 @@ NCB_API int ncb_sample_rows_min_p_device(const void* d_logits, int dtype, int ro
  * [out_features, rank_s], x [rows, in_features], all of the handle's dtype
  * (NCB_DTYPE_F16 or NCB_DTYPE_BF16). Products are summed in fp32 and rounded
  * once, to the output's type; scale_s A_s x_n goes into the second product as the
- * sum of two values of the handle's type (2^-16 of it or less is lost). No sum's
- * order depends on timing: the same call gives the same bits. A row whose adapter
+ * sum of two values of the handle's type (2^-16 of it or less is lost), of three
+ * where bf16 is projected to fp32 (2^-24). No sum's order depends on timing: the same call gives the same bits. A row whose adapter
  * holds a NaN or an infinity, or whose scale_s A_s x_n is not finite in the
  * handle's type (fp16: beyond 65504), comes back as NaN; no other row of the call
  * is touched by it.

@@ -7,8 +7,10 @@
 // read once. The adapters are part of the same sums, a longer inner axis:
 //   out^T += B_e U_e^T   for each entry e = (16 ranks of a slot, a block of rows),
 // U_e holding u_n = scale_s A_s x_n for the rows n of the block that name the slot
-// and zeros for the others, split into two 16-bit values, u = hi + lo, each with
-// its own product (one would round u to 8 bits of bf16).
+// and zeros for the others, split into 16-bit values, each with its own product (one
+// would round u to 8 bits of bf16): two, u = hi + lo, 16 bits, where the output is
+// rounded to fewer anyway, and three for bf16 with an fp32 output (with two the
+// result was 1.2e-6 off, more than all of the sums).
 //
 // Tiles of up to AH_SINGLE rows have one block, the tile. Larger tiles are sorted by
 // slot first (adapter_sort_kernel copies x in that order) and cut into blocks of 32
@@ -49,10 +51,9 @@ constexpr int AH_MAX_STAGES = 12;
 constexpr int AH_SMEM = 208 * 1024;  // stages; leaves room for a shrink CTA on the SM
 constexpr int AH_EPILOGUE = 8;    // warps that write results
 constexpr int AH_THREADS = (AH_EPILOGUE + 2) * 32;  // and a copying and a multiplying one
-constexpr int AH_PIECE = 4;       // stages added up in TMEM for an fp32 output
+constexpr int AH_PIECE = 8;       // stages added up in TMEM for an fp32 output
 constexpr int AH_SINGLE = 64;     // rows per tile up to which single CTAs work, unsorted
 constexpr int AH_BLOCK = 32;      // rows per block of larger tiles
-__host__ __device__ constexpr int ah_per(int group) { return group == 1 ? 2 : 4; }  // adapter entries per stage
 
 struct AhArgs {
   const void* x;
@@ -62,12 +63,13 @@ struct AhArgs {
   const int32_t* ids;
   const void* a;        // [slots][16 slices][kpad]
   int block, bh;        // rows per block, of it per CTA
+  int parts, per;       // 16-bit values that make up u; entries per stage of the head
   void* x_sorted;       // [rows][kpad]
   int4* info;           // [tiles_n][AH_NT] by row: place, first entry, first and last place of its slot
   int32_t* order;       // [tiles_n][AH_NT] by place: row of the tile; NULL: as they come
   const int32_t* ranks; // per slot; 0: empty, < 0: |rank|, and B holds a non-finite value
   const float* scales;
-  void* u;              // [tiles_n][block / bh][max_entries][hi, lo][bh][16]
+  void* u;              // [tiles_n][block / bh][max_entries][parts][bh][16]
   int2* entries;        // [tiles_n][max_entries] slot * slices + slice, first place
   int32_t* counts;      // [tiles_n]
   int max_entries, opad;
@@ -94,8 +96,8 @@ __host__ __device__ __forceinline__ int64_t ah_at(int64_t r, int j) {
 // value of B that is not finite would reach every row of a tile (0 times NaN);
 // it is stored as 0 and the slot marked, and the slot's own rows come out as NaN.
 template <typename E>
-__global__ void adapter_pack_kernel(E* a, E* b, int32_t* ranks, float* scales, int slot, int in,
-                                    int kpad, int out, int opad, int slices, const E* sa,
+__global__ void adapter_pack_kernel(E* a, E* b, int32_t* ranks, int slot, int in, int kpad,
+                                    int out, int opad, int slices, const E* sa,
                                     int64_t lda, const E* sb, int64_t ldb, int rank) {
   const int64_t na = (int64_t)slices * 16 * kpad, nb = (int64_t)slices * opad * 16;
   const int64_t t0 = blockIdx.x * (int64_t)blockDim.x + threadIdx.x, dt = (int64_t)gridDim.x * blockDim.x;
@@ -261,14 +263,15 @@ __global__ void __launch_bounds__(AU_THREADS, 4) adapter_shrink_kernel(const AhA
   const int r = blockIdx.x, tile = blockIdx.y, n0 = tile * g.nt;
   int mine;
   const int slot = as_slot(g, n0 + r, &mine);
-  E* u = static_cast<E*>(g.u) + (int64_t)tile * g.max_entries * 2 * g.block * 16;
-  // where an entry's part of the block's row `at` lies, hi; lo is bh rows further
+  E* u = static_cast<E*>(g.u) + (int64_t)tile * g.max_entries * g.parts * g.block * 16;
+  // an entry's share of the block that holds row `at`; each part is bh rows
   auto row_of = [&](int e, int at) {
-    return u + ((int64_t)(at / g.bh) * g.max_entries + e) * 2 * g.bh * 16;
+    return u + ((int64_t)(at / g.bh) * g.max_entries + e) * g.parts * g.bh * 16;
   };
-  auto clear = [&](int e, int at, int quarter) {  // 16 bytes of the row's hi and lo
-    *reinterpret_cast<uint4*>(row_of(e, at) + (quarter & 2 ? g.bh * 16 : 0) + at % g.bh * 16 +
-                              (quarter & 1) * 8) = make_uint4(0, 0, 0, 0);
+  auto clear = [&](int e, int at, int half) {  // the half of the row, in every part
+    for (int p = 0; p < g.parts; ++p)
+      *reinterpret_cast<uint4*>(row_of(e, at) + p * g.bh * 16 + at % g.bh * 16 + half * 8) =
+          make_uint4(0, 0, 0, 0);
   };
   int own, next, place;  // the row's first entry, how far to the next 16 ranks', the row in it
   const E* x = static_cast<const E*>(g.x) + (int64_t)(n0 + r) * g.ldx;
@@ -284,9 +287,9 @@ __global__ void __launch_bounds__(AU_THREADS, 4) adapter_shrink_kernel(const AhA
       for (int j = 0; j < mine; ++j) {
         const int front = info.z % AH_BLOCK, back = AH_BLOCK - 1 - info.w % AH_BLOCK;
         const int e = info.y + j * next;
-        for (int i = t; i < 4 * front; i += AU_THREADS) clear(e, i >> 2, i & 3);
-        for (int i = t; i < 4 * back; i += AU_THREADS)
-          clear(e + b1 - b0, AH_BLOCK - back + (i >> 2), i & 3);
+        for (int i = t; i < 2 * front; i += AU_THREADS) clear(e, i >> 1, i & 1);
+        for (int i = t; i < 2 * back; i += AU_THREADS)
+          clear(e + b1 - b0, AH_BLOCK - back + (i >> 1), i & 1);
       }
   } else {
     const int none = 0x7FFFFFFF;
@@ -322,8 +325,8 @@ __global__ void __launch_bounds__(AU_THREADS, 4) adapter_shrink_kernel(const AhA
           entries[mine_at + i] = make_int2((kt >> 8) * g.slices + i, 0);
       if (t == 0) g.counts[tile] = count;
     }
-    for (int i = t; i < 4 * count; i += AU_THREADS)
-      if (i >> 2 < own || i >> 2 >= own + mine) clear(i >> 2, r, i & 3);
+    for (int i = t; i < 2 * count; i += AU_THREADS)
+      if (i >> 1 < own || i >> 1 >= own + mine) clear(i >> 1, r, i & 1);
     if (!mine) return;
   }
   for (int slice = 0; slice < mine; ++slice) {
@@ -368,10 +371,12 @@ __global__ void __launch_bounds__(AU_THREADS, 4) adapter_shrink_kernel(const AhA
     v *= g.scales[slot];
     E hi = E(v);
     if (g.ranks[slot] < 0 || !(fabsf((float)hi) < INFINITY)) hi = E(NAN);
-    const E lo = E(v - (float)hi);
     E* to = row_of(own + slice * next, place) + ah_at(place % g.bh, t);
-    to[0] = hi;
-    to[(int64_t)g.bh * 16] = lo;
+    for (int p = 0; p < g.parts; ++p) {  // what the parts before have left, rounded
+      to[(int64_t)p * g.bh * 16] = hi;
+      v -= (float)hi;
+      hi = E(v);
+    }
   }
   __syncthreads();
   }
@@ -563,7 +568,6 @@ __global__ void __launch_bounds__(AH_THREADS, 1)
   ah_all_sync<CG>();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = s_tmem;
-  constexpr int PER = ah_per(CG);
   const int steps = (g.in + AH_BK - 1) / AH_BK;
   const int piece = CPT ? AH_PIECE : steps;  // stages added up in TMEM
   const int pieces = (steps + piece - 1) / piece;
@@ -608,15 +612,15 @@ __global__ void __launch_bounds__(AH_THREADS, 1)
           if (lane < count) mine = __ldcg(entries + lane);
         }
       }
-      for (int e = 0; e < count; e += PER) {
+      for (int e = 0; e < count; e += g.per) {
         if (e && (e & 31) == 0 && e + lane < count) mine = __ldcg(entries + e + lane);
         if (!(ok = ah_wait(empty + 8 * s, phase ^ 1))) break;
-        const int several = min(PER, count - e);
+        const int several = min(g.per, count - e);
         const uint32_t a = stage0 + s * stage_bytes, bar = full + 8 * s;
         if (lane == 0) {  // U of a whole stage at once, whether it is full or not
-          if (rank == 0) ah_expect(bar, CG * (several * AH_BM * 32 + PER * g.bh * 64));
-          ah_copy<CG>(a + AH_A_BYTES, &map_u, bar, 0,
-                      (int)(((int64_t)(n * CG + rank) * g.max_entries + e) * g.bh / 8));
+          if (rank == 0) ah_expect(bar, CG * (several * AH_BM * 32 + g.per * g.parts * g.bh * 32));
+          ah_copy<CG>(a + g.per * AH_BM * 32, &map_u, bar, 0,
+                      (int)(((int64_t)(n * CG + rank) * g.max_entries + e) * g.parts * g.bh / 16));
         }
         for (int j = 0; j < several; ++j) {
           const int z = __shfl_sync(0xffffffffu, mine.x, (e & 31) + j);
@@ -678,19 +682,20 @@ __global__ void __launch_bounds__(AH_THREADS, 1)
                 if (lane < count) mine = __ldcg(&entries[lane].y);
               }
             }
-            for (int e = 0; e < count; e += PER) {
+            for (int e = 0; e < count; e += g.per) {
               if (e && (e & 31) == 0 && e + lane < count) mine = __ldcg(&entries[e + lane].y);
               if (!(ok = ah_wait(full + 8 * s, phase))) break;
               asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-              const int several = min(PER, count - e);
+              const int several = min(g.per, count - e);
               const uint32_t base = stage0 + s * stage_bytes;
               for (int j = 0; j < several; ++j) {
                 const int place = __shfl_sync(0xffffffffu, mine, (e & 31) + j);
                 if (lane == 0) {
                   const uint64_t a = ah_operand(base + j * AH_BM * 32, 32);
-                  const uint32_t u = base + AH_A_BYTES + j * g.bh * 64;
-                  ah_multiply<CG>(acc + place, a, ah_operand(u, 32), g.idesc_u, true);
-                  ah_multiply<CG>(acc + place, a, ah_operand(u + g.bh * 32, 32), g.idesc_u, true);
+                  for (int p = 0; p < g.parts; ++p)
+                    ah_multiply<CG>(acc + place, a,
+                                    ah_operand(base + g.per * AH_BM * 32 + (j * g.parts + p) * g.bh * 32, 32),
+                                    g.idesc_u, true);
                 }
               }
               if (lane == 0) ah_commit<CG>(empty + 8 * s);
@@ -1002,7 +1007,7 @@ NCB_API int ncb_adapter_head_create(int device, int dtype, int in_features, int 
   const size_t per = (size_t)h->slots * h->slices * 16;
   const size_t o_a = carve(per * h->kpad * 2), o_b = carve(per * h->opad * 2);
   const size_t o_x = carve((size_t)max_rows * h->kpad * 2);
-  const size_t o_u = carve(tiles * most * 2 * nvs::AH_SINGLE * 16 * 2);  // the larger block
+  const size_t o_u = carve(tiles * most * 3 * nvs::AH_SINGLE * 16 * 2);  // the larger block
   const size_t o_e = carve(tiles * most * sizeof(int2)), o_c = carve(tiles * 4);
   const size_t o_i = carve(tiles * nvs::AH_NT * sizeof(int4)), o_o = carve(tiles * nvs::AH_NT * 4);
   const size_t o_s = carve((size_t)h->slots * 4), o_r = carve((size_t)h->slots * 4);
@@ -1145,6 +1150,10 @@ NCB_API int ncb_adapter_head_project_device(NcbAdapterHead* h, const void* d_x, 
   const bool sorted = g.ids && group == 2;
   g.block = group == 2 ? nvs::AH_BLOCK : g.nt;
   g.bh = g.block / group;
+  g.parts = h->dtype == NCB_DTYPE_BF16 && out_dtype == NCB_DTYPE_F32 ? 3 : 2;
+  // a stage holds 4 KiB of B for each entry and, behind them, the entries' U: 4 * 4 KiB
+  // and 4 * 3 * 16 * 32 bytes of 32 KiB, or 2 * 4 KiB and 2 * 3 * bh * 32 of 16 KiB + bh * 128
+  g.per = group == 2 ? 4 : 2;
   g.max_entries = (h->slots < nvs::AH_NT ? h->slots : nvs::AH_NT) * h->slices +
                   nvs::AH_NT / nvs::AH_BLOCK * h->slices;
   g.a = h->a;
@@ -1197,8 +1206,8 @@ NCB_API int ncb_adapter_head_project_device(NcbAdapterHead* h, const void* d_x, 
     return ncb_record_status(NCB_ERROR_LAUNCH_FAILED);
   if (!ah_map(&m.x, h->dtype, sorted ? h->x_own : d_x, h->in, rows, sorted ? h->kpad : ldx,
               nvs::AH_BK, g.nh, CU_TENSOR_MAP_SWIZZLE_128B) ||
-      (g.ids && !ah_map(&m.u, h->dtype, h->u, 256, (int64_t)g.tiles_n * g.max_entries * 2 * g.block / 16,
-                        256, 256, nvs::ah_per(group) * g.bh / 8, CU_TENSOR_MAP_SWIZZLE_NONE)))
+      (g.ids && !ah_map(&m.u, h->dtype, h->u, 256, (int64_t)g.tiles_n * g.max_entries * g.parts * g.block / 16,
+                        256, 256, g.per * g.parts * g.bh / 16, CU_TENSOR_MAP_SWIZZLE_NONE)))
     return ncb_record_status(NCB_ERROR_LAUNCH_FAILED);
   const bool wide = out_dtype == NCB_DTYPE_F32;
   if (h->dtype == NCB_DTYPE_BF16)

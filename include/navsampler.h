@@ -375,10 +375,10 @@ NCB_API int ncb_sample_rows_min_p_device(const void* d_logits, int dtype, int ro
  * (NCB_DTYPE_F16 or NCB_DTYPE_BF16). Products are summed in fp32 and rounded
  * once, to the output's type; scale_s A_s x_n goes into the second product as the
  * sum of two values of the handle's type (2^-16 of it or less is lost), of three
- * where bf16 is projected to fp32 (2^-24). No sum's order depends on timing: the same call gives the same bits. A row whose adapter
- * holds a NaN or an infinity, or whose scale_s A_s x_n is not finite in the
- * handle's type (fp16: beyond 65504), comes back as NaN; no other row of the call
- * is touched by it.
+ * where bf16 is projected to fp32 (2^-24). No sum's order depends on timing: the
+ * same call gives the same bits. A row whose adapter holds a NaN or an infinity,
+ * or whose scale_s A_s x_n is not finite in the handle's type (fp16: beyond
+ * 65504), comes back as NaN; no other row of the call is touched by it.
  *
  * The handle owns packed copies of the adapters and its scratch; like a
  * sampler it is single-stream: calls on one handle must not overlap on the GPU

@@ -868,7 +868,7 @@ int ah_pack(NcbAdapterHead* h, int slot, const void* a, int64_t lda, const void*
             int rank, float scale, cudaStream_t st) {
   nvs::adapter_slot_kernel<<<1, 1, 0, st>>>(h->ranks, h->scales, slot, rank, scale);
   nvs::adapter_pack_kernel<E><<<4 * h->num_sms, 256, 0, st>>>(
-      static_cast<E*>(h->a), static_cast<E*>(h->b), h->ranks, h->scales, slot, h->in, h->kpad,
+      static_cast<E*>(h->a), static_cast<E*>(h->b), h->ranks, slot, h->in, h->kpad,
       h->out, h->opad, h->slices, static_cast<const E*>(a), lda, static_cast<const E*>(b), ldb, rank);
   return ah_launched();
 }

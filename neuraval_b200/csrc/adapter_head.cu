@@ -16,13 +16,18 @@
 // slot first (adapter_sort_kernel copies x in that order) and cut into blocks of 32
 // rows, so that a slot's entries cover little more than its own rows: with whole
 // tiles as blocks, 32 slots of 16 ranks took a quarter of the tensor cores' time
-// (256x4096x128256: 284 us, without adapters 234).
+// (256x4096x128256: 284 us, without adapters 234). The sort costs
+// a launch that nothing hides, and a pair has half the copies in flight: 12 slots of
+// 16 ranks, single CTAs against pairs: 80x4096x128256 194 and 203 us, 96 rows 198 and
+// 197 (fp32 207 and 223), 128 rows 217 and 211; 96x2048x32000 40 and 46.
 //
 // adapter_shrink_kernel computes u while the head multiplies its first tile; the
 // head waits for it only before the first entry (programmatic dependent launch).
 //
-// Up to about 256 rows the head is bound by the weight's bytes, beyond by the
-// tensor cores and the power they draw.
+// Up to about 256 rows the head is bound by the weight's bytes (32x4096x128256, 8
+// slots of 16 ranks: 176 us, 6.2 TB/s), beyond by the tensor cores and the power they
+// draw (512x4096x151936, 16 slots of 32 ranks: 582 us alone, 1.1 PFLOP/s, 700 us in
+// a long loop whose clock sinks to 1 GHz).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -52,8 +57,20 @@ constexpr int AH_SMEM = 208 * 1024;  // stages; leaves room for a shrink CTA on 
 constexpr int AH_EPILOGUE = 8;    // warps that write results
 constexpr int AH_THREADS = (AH_EPILOGUE + 2) * 32;  // and a copying and a multiplying one
 constexpr int AH_PIECE = 8;       // stages added up in TMEM for an fp32 output
-constexpr int AH_SINGLE = 64;     // rows per tile up to which single CTAs work, unsorted
+constexpr int AH_SINGLE = 96;     // rows per tile up to which single CTAs work, unsorted
 constexpr int AH_BLOCK = 32;      // rows per block of larger tiles
+constexpr int AH_PARTS = 3;       // 16-bit values that make up u, at most
+
+// Adapter entries per stage. A stage, AH_A_BYTES + nh * 128 bytes, holds 4 KiB of B for
+// each and, behind them, the entries' U, AH_PARTS * bh * 32 bytes each. (Copies cost
+// about the same whatever their size, so pairs take four entries with one copy of U.)
+constexpr int ah_per(int group) { return group == 2 ? 4 : 2; }
+constexpr bool ah_fits(int group, int nh, int bh) {
+  return ah_per(group) * (AH_BM * 32 + AH_PARTS * bh * 32) <= AH_A_BYTES + nh * 128;
+}
+// (single CTAs: bh = nh, and the entries' bytes grow by 192 nh, the stage's by 128 nh)
+static_assert(ah_fits(1, AH_SINGLE, AH_SINGLE), "entries of a single CTA");
+static_assert(ah_fits(2, (AH_SINGLE + 32) / 32 * 32 / 2, AH_BLOCK / 2), "entries of the smallest pair");
 
 struct AhArgs {
   const void* x;
@@ -1007,7 +1024,7 @@ NCB_API int ncb_adapter_head_create(int device, int dtype, int in_features, int 
   const size_t per = (size_t)h->slots * h->slices * 16;
   const size_t o_a = carve(per * h->kpad * 2), o_b = carve(per * h->opad * 2);
   const size_t o_x = carve((size_t)max_rows * h->kpad * 2);
-  const size_t o_u = carve(tiles * most * 3 * nvs::AH_SINGLE * 16 * 2);  // the larger block
+  const size_t o_u = carve(tiles * most * nvs::AH_PARTS * nvs::AH_SINGLE * 16 * 2);  // the larger block
   const size_t o_e = carve(tiles * most * sizeof(int2)), o_c = carve(tiles * 4);
   const size_t o_i = carve(tiles * nvs::AH_NT * sizeof(int4)), o_o = carve(tiles * nvs::AH_NT * 4);
   const size_t o_s = carve((size_t)h->slots * 4), o_r = carve((size_t)h->slots * 4);
@@ -1150,10 +1167,8 @@ NCB_API int ncb_adapter_head_project_device(NcbAdapterHead* h, const void* d_x, 
   const bool sorted = g.ids && group == 2;
   g.block = group == 2 ? nvs::AH_BLOCK : g.nt;
   g.bh = g.block / group;
-  g.parts = h->dtype == NCB_DTYPE_BF16 && out_dtype == NCB_DTYPE_F32 ? 3 : 2;
-  // a stage holds 4 KiB of B for each entry and, behind them, the entries' U: 4 * 4 KiB
-  // and 4 * 3 * 16 * 32 bytes of 32 KiB, or 2 * 4 KiB and 2 * 3 * bh * 32 of 16 KiB + bh * 128
-  g.per = group == 2 ? 4 : 2;
+  g.parts = h->dtype == NCB_DTYPE_BF16 && out_dtype == NCB_DTYPE_F32 ? nvs::AH_PARTS : 2;
+  g.per = nvs::ah_per(group);
   g.max_entries = (h->slots < nvs::AH_NT ? h->slots : nvs::AH_NT) * h->slices +
                   nvs::AH_NT / nvs::AH_BLOCK * h->slices;
   g.a = h->a;

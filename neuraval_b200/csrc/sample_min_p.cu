@@ -7,15 +7,19 @@
 //
 // Every set is a prefix of the order, so a row needs no sort, only the places
 // where a count (top_k), a value (min_p) or a mass (top_p, the draw) is crossed.
-// A row belongs to a cluster of 1..8 CTAs (more CTAs for few rows), which pass over
-// it two or three times; all passes but the first mostly read L2. CTA 0 decides, the
-// others carry out its commands:
-//   1. maximum and least finite value (NaN and +inf show in a NaN-propagating
-//      maximum), and each thread's own maximum;
-//   2. few values wanted (the usual options): the k-th largest of the threads'
-//      maxima is a lower bound of the k-th value, min-p has one of its own. What is
-//      above is gathered into one list, sorted by (x, id), and everything is decided
-//      on 64-bit prefix sums of the list.
+// Rows of 16-bit values have a kernel of their own, further down, which counts each
+// value; this is the one for fp32 rows. A row belongs to a cluster of 1..8 CTAs (more
+// CTAs for few rows). CTA 0 decides, the others carry out its commands:
+//   1. few values wanted (the usual options): each thread's maximum of the first
+//      quarter or half of the row; the k-th largest of them is a lower bound of the
+//      k-th value, min-p has one of its own. The rest is read once, what is above the
+//      bound listed (each CTA its own, then one list), sorted by (x, id), and
+//      everything is decided on 64-bit prefix sums of the list. The row crosses HBM
+//      once: 256x128256 takes 65 us, 2.0 TB/s, its floor being 20; what is left
+//      is the list's sort and the cluster's and the block's barriers, of which two
+//      CTAs to an SM hide a part.
+//   2. Otherwise the maximum and the least finite value (NaN and +inf show in a
+//      NaN-propagating maximum) of all of it; the passes that follow mostly read L2.
 //   3. Otherwise, or where the list overflows: a histogram of counts over SP_BINS
 //      equal steps of x below the maximum (integers: their order does not matter).
 //      It gives the bin of the k-th value exactly, and about where the masses are
@@ -29,7 +33,9 @@
 //
 // Keeping a cluster's slices of the row in shared memory, for one read in all, was
 // slower: it leaves two CTAs per SM in long chains of small steps, and more of them
-// per row to synchronise (1024x151936: 2.3 ms, now NOWFLAT).
+// per row to synchronise (1024x151936 with top-p alone: 2.3 ms, now 0.94, of which
+// the 64-bit weights of the exact pass are the largest part: it issues about 30
+// operations per value).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -1925,6 +1931,8 @@ int sp_launch(const nvs::SpArgs& a, int rows, int device, int num_sms, cudaStrea
   const int granules = (a.vocab + n - 1) / n + 1;
   if constexpr (sizeof(E) == 2) {
     // as many CTAs to a row as its values need, then as fill the GPU, one per SM
+    // (their counters take its shared memory). Each counts up to 65535 values: 128256
+    // values need two, which 256 rows' 512 CTAs pay for with 3.5 waves.
     const int values = granules * n;
     int ranks = values <= nvs::SQ_ALONE ? 1 : 2;
     while (ranks < nvs::SP_CLUSTER &&
@@ -1944,7 +1952,9 @@ int sp_launch(const nvs::SpArgs& a, int rows, int device, int num_sms, cudaStrea
     }
   }
   // as many CTAs to a row as fill the GPU twice over, while each has two granules for
-  // every thread
+  // every thread: a cluster's barriers cost more than they win where rows alone fill
+  // it (256x128256: 65 us with one CTA to a row, 81 with two, 119 with four;
+  // 1x32000: 27 us with one, 23 with eight)
   int ranks = 1;
   while (ranks < nvs::SP_CLUSTER && (int64_t)rows * ranks * 2 <= 2 * num_sms &&
          granules / ranks >= 2 * nvs::SP_NT)

@@ -145,6 +145,21 @@ def test_ranks_and_many_adapters(ranks, rows):
         check(c.run(h), *c.want())
 
 
+@pytest.mark.parametrize("out", ["f32", "same"])
+@pytest.mark.parametrize("rows", [63, 65, 80, 81, 96, 97, 128, 129, 192, 194])
+def test_sizes_where_the_tiles_change(rows, out):
+    """Row counts on both sides of each change of tile, with many adapters and mixed ranks."""
+    ranks = [16, 1, 17, 48] * 9 + [128]
+    ids = np.random.default_rng(rows).integers(-1, len(ranks), rows)
+    c = Case(rows, 264, 777, ranks, ids, "bf16", rows, whole=True)
+    with c.head() as h:
+        got, want = c.run(h, "f32" if out == "f32" else "bf16"), c.want()[0].float()
+        assert (got == want.to(got.dtype)).all()
+    c = Case(rows, 264, 777, ranks, ids, "bf16", rows + 1)
+    with c.head() as h:
+        check(c.run(h, "f32" if out == "f32" else "bf16"), *c.want())
+
+
 def test_ids_without_an_adapter():
     """-1, ids outside the slots, empty and cleared slots: the shared projection alone."""
     ids = [-1, 0, 5, -2 ** 31, 2 ** 31 - 1, 2, 1, 3, 4, 0]

@@ -16,10 +16,10 @@
 // slot first (adapter_sort_kernel copies x in that order) and cut into blocks of 32
 // rows, so that a slot's entries cover little more than its own rows: with whole
 // tiles as blocks, 32 slots of 16 ranks took a quarter of the tensor cores' time
-// (256x4096x128256: 284 us, without adapters 234). The sort costs
-// a launch that nothing hides, and a pair has half the copies in flight: 12 slots of
-// 16 ranks, single CTAs against pairs: 80x4096x128256 194 and 203 us, 96 rows 198 and
-// 197 (fp32 207 and 223), 128 rows 217 and 211; 96x2048x32000 40 and 46.
+// (256x4096x128256: 284 us, without adapters 234). The sort costs a launch that
+// nothing hides. Single CTAs against pairs, 12 slots of 16 ranks (16 for 128 rows):
+// 80x4096x128256 194 and 203 us, 96 rows 198 and 197 (fp32 207 and 223), 128 rows 217
+// and 211; 96x2048x32000 40 and 46.
 //
 // adapter_shrink_kernel computes u while the head multiplies its first tile; the
 // head waits for it only before the first entry (programmatic dependent launch).

@@ -47,6 +47,7 @@
 #include <cstdint>
 
 #include "navsampler.h"
+#include "sample_search.cuh"
 
 int ncb_record_status(int st);
 
@@ -140,14 +141,6 @@ struct SpShared {
 extern __shared__ uint4 sp_raw[];
 __device__ __forceinline__ SpShared& sp_shared() { return *reinterpret_cast<SpShared*>(sp_raw); }
 
-// Floats in order as unsigned integers; -0 counts as +0.
-__device__ __forceinline__ uint32_t sp_key(float v) {
-  const uint32_t b = __float_as_uint(v + 0.0f);
-  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
-}
-__device__ __forceinline__ float sp_value(uint32_t k) {
-  return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
-}
 // A window's greatest key as a value. (No value has the key of -0; as a float it would
 // take +0 with it.)
 __device__ __forceinline__ float sp_edge(uint32_t k) {
@@ -435,15 +428,8 @@ struct SpOptions {
   }
 };
 
-// The least value that min-p keeps: w >= m  <=>  x >= max + T ln m.
 __device__ float sp_least_kept(float mx, float T, float min_p, double inv_t) {
-  if (!(min_p > 0.0f)) return -FLT_MAX;
-  const double edge = log((double)min_p), at = (double)mx + edge * (double)T;
-  float least = at > -(double)FLT_MAX ? (float)at : -FLT_MAX;
-  auto kept = [&](float v) { return ((double)v - (double)mx) * inv_t >= edge; };
-  while (least < mx && !kept(least)) least = nextafterf(least, INFINITY);
-  while (least > -FLT_MAX && kept(nextafterf(least, -INFINITY))) least = nextafterf(least, -INFINITY);
-  return least;
+  return sp_least_kept(mx, T, min_p, inv_t, [] {});
 }
 
 // What a value of the row means. The passes work on a copy of their own: behind a

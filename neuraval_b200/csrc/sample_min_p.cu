@@ -114,7 +114,7 @@ struct SpPart {
 
 struct SpShared {
   uint4 hist4[SP_BINS / 4];  // counts; in CTA 0, once merged, the counts before each bin
-  float4 some4[SP_SOME / 4]; // a value of each filled bin, of the first bins
+  uint4 some4[SP_SOME / 4];  // the greatest key of each filled bin, of the first bins
   alignas(16) float mass[SP_BINS + 4];  // CTA 0, once merged: about the mass before each bin
   unsigned long long list[SP_WINDOWS * SP_CAP];
   SpCmd cmd;
@@ -537,7 +537,8 @@ struct SpRow {
         if (v[e] > -INFINITY) {
           const int b = k.bin(v[e]);
           atomicAdd(reinterpret_cast<int*>(s.hist4) + b, 1);
-          if (b < SP_SOME) reinterpret_cast<float*>(s.some4)[b] = v[e];  // any of them
+          // (of some value: the windows that are guessed from it must not depend on timing)
+          if (b < SP_SOME) atomicMax(reinterpret_cast<uint32_t*>(s.some4) + b, sp_key(v[e]));
         }
     });
   }
@@ -799,6 +800,11 @@ struct SpRow {
       }
     }
   }
+  __device__ __forceinline__ void clear() {
+    SpShared& s = sp_shared();
+    s.hist4[threadIdx.x] = make_uint4(0, 0, 0, 0);
+    if (threadIdx.x < SP_SOME / 4) s.some4[threadIdx.x] = make_uint4(0, 0, 0, 0);
+  }
   __device__ __noinline__ void carry_out(const SpCmd& m) {
     SpShared& s = sp_shared();
     if (m.op == SP_FIRST) {
@@ -808,7 +814,7 @@ struct SpRow {
     }
     if (m.op == SP_PASS) pass(m);
     if (m.op == SP_HIST) {
-      s.hist4[threadIdx.x] = make_uint4(0, 0, 0, 0);
+      clear();
       __syncthreads();
       if (m.shift < 0) hist_by_value();
       else hist_by_key(m);
@@ -857,13 +863,13 @@ struct SpRow {
     for (int r = 0; r < SP_CLUSTER; ++r)
       if (r < ranks) {
         const uint4 c = of(r).hist4[threadIdx.x];
-        const float4 f = by_value && 4 * threadIdx.x < SP_SOME ? of(r).some4[threadIdx.x]
-                                                              : make_float4(0.f, 0.f, 0.f, 0.f);
+        const uint4 f = by_value && 4 * threadIdx.x < SP_SOME ? of(r).some4[threadIdx.x]
+                                                              : make_uint4(0, 0, 0, 0);
         const uint32_t ci[4] = {c.x, c.y, c.z, c.w};
-        const float fi[4] = {f.x, f.y, f.z, f.w};
+        const uint32_t fi[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (ci[j]) x[j] = fi[j];
+          if (ci[j]) x[j] = sp_value(fi[j]);
           n[j] += (int)ci[j];
         }
       }
@@ -1054,7 +1060,7 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
   R.cl.barrier_arrive();  // this CTA runs: the others may write into it
   R.sl.set(static_cast<const E*>(a.logits) + (int64_t)row * a.ld, a.vocab, R.rank, a.per);
   R.T = T;
-  s.hist4[t] = make_uint4(0, 0, 0, 0);
+  R.clear();
   if (t < SP_WINDOWS) s.n_list[t] = 0;
   // ---- maximum, least finite value; where few values are wanted, of a part of the row first --------
   const bool bounded = !greedy && k_asked > 0 && k_asked <= min(SP_BOUNDED, SP_NT * R.ranks / 2);

@@ -1036,6 +1036,7 @@ struct SpWindow {
   uint32_t klo0, khi0;  // by_key: keys between which the crossing is known to lie,
   double above0;        //   and the mass above them
   bool gather;
+  SpSpan span;          // the values of which the crossing is one
 };
 
 template <typename E>
@@ -1238,8 +1239,10 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
         win[w].klo = s.tops[SP_WINDOWS + w] + 1;
       }
   };
-  for (int w = 0; w < SP_WINDOWS; ++w)
+  for (int w = 0; w < SP_WINDOWS; ++w) {
+    win[w].span = {0, k};  // all three are in K
     if (!found[w]) set_bins(w);
+  }
 
   // After a histogram of the keys in [lo, hi] (whose mass above is `above`, values
   // above n_above): the window around the crossing of `want` (a mass, or a count).
@@ -1264,7 +1267,7 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
     if (count) {
       a1 = z1 = R.bin_of_count((int)want - n_above, n);
     } else {
-      const int b = R.bin_of_mass((float)(want - above), n);
+      const int b = R.bin_of_mass((float)fmax(want - above, 0.0), n);
       R.window_of(b, 0, SP_BINS - 1, n, &a1, &z1);
     }
     win[w].by_key = true;
@@ -1279,8 +1282,8 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
   int token = -1;
   float token_value = 0.0f;
   int nth = -1;  // >= 0: the token is this occurrence of token_value
-  // Each turn finds a crossing or leaves it fewer values (a neighbouring window, or
-  // the part of one that holds it), so the loop ends; the limit is a guard.
+  // Each turn finds a crossing or excludes values from it for good (sp_turn: a window, or
+  // all but one), so the loop ends; the limit is a guard.
   for (int turn = 0; !found[SP_D] && turn < SP_TURNS; ++turn) {
     bool first = true;  // all windows are runs of bins: the first pass will do
     for (int w = 0; w < SP_WINDOWS; ++w) first = first && (found[w] || !(win[w].by_key || win[w].weigh));
@@ -1351,53 +1354,46 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
       SpWindow& v = win[w];
       const double ab = p.above(w);
       auto past = [&](double x) { return beyond ? x > want : x >= want; };
-      const bool up = past(ab) && p.n_above(w) > 0;
-      double in = p.in(w), wt = 0.0, sum[1] = {0.0};
-      const int n = p.n_in(w);
+      const int n = p.n_in(w), above = p.n_above(w);
+      const bool up = past(ab) && above > v.span.lo;
+      double in = p.in(w), sum[1] = {0.0};
       if (!up && v.gather) {  // the list says what is in the window
         double each[1];
         sp_sort(s.list + w * SP_CAP, n);
         R.template prefixes<1>(s.list + w * SP_CAP, n, each, sum);
         if (first) in = n ? R.template sum_at<1>(sum, n - 1) : 0.0;
       }
-      const bool down = !up && in >= 0.0 && !past(ab + in);
-      if (!up && !down && v.gather) {
-        *at = min(R.template count<1>([&](int) { return t < n && !past(ab + sum[0]); }), n - 1);
-        *mass = ab + R.template sum_at<1>(sum, *at);
-        return 0;
-      }
-      if (!up && !down && !v.gather && v.klo == v.khi) {  // equal values
-        wt = R.k.weight_any(sp_value(v.klo));
-        double j = floor((want - ab) / wt);  // values passed before, give or take one
-        if (j > 0.0 && past(ab + j * wt)) j -= 1.0;
-        if (!past(ab + (j + 1.0) * wt)) j += 1.0;
-        *at = (int)fmin(fmax(j, 0.0), (double)(n - 1));
-        *mass = ab + (*at + 1.0) * wt;
-        return 0;
-      }
       if (first && !v.gather && in < 0.0 && !up) {  // too many different values: their mass first
         v.weigh = true;
         return 1;
       }
-      if (!v.by_key) {
-        if (up && v.a > 0) {  // the bins just before
-          need_bins();
-          const int b = v.a - 1;
-          R.window_of(b, 0, b, total, &v.a, &v.z);
-          set_bins(w);
-        } else if (down && v.z < last) {
-          need_bins();
-          const int b = v.z + 1;
-          R.window_of(b, b, last, total, &v.a, &v.z);
-          set_bins(w);
-        } else {
-          divide(w, v.klo, v.khi, ab, p.n_above(w), want, false);
-        }
-        return 1;
+      const int way = sp_turn(v.span, above, n, past(ab), past(ab + in));
+      const int front = v.span.lo - above, back = v.span.hi - 1 - above;  // SP_HERE: places it may have
+      if (way == SP_HERE && v.gather) {
+        *at = min(max(R.template count<1>([&](int) { return t < n && !past(ab + sum[0]); }), front), back);
+        *mass = ab + R.template sum_at<1>(sum, *at);
+        return 0;
       }
-      if (up && v.khi < v.khi0) divide(w, v.khi + 1, v.khi0, v.above0, 0, want, false);
-      else if (down && v.klo > v.klo0) divide(w, v.klo0, v.klo - 1, ab + in, 0, want, false);
-      else divide(w, v.klo, v.khi, ab, p.n_above(w), want, false);
+      if (way == SP_HERE && v.klo == v.khi) {  // equal values
+        const double wt = R.k.weight_any(sp_value(v.klo));
+        double j = floor((want - ab) / wt);  // values passed before, give or take one
+        if (j > 0.0 && past(ab + j * wt)) j -= 1.0;
+        if (!past(ab + (j + 1.0) * wt)) j += 1.0;
+        *at = (int)fmin(fmax(j, (double)front), (double)back);
+        *mass = ab + (*at + 1.0) * wt;
+        return 0;
+      }
+      if (way == SP_HERE) {
+        divide(w, v.klo, v.khi, ab, above, want, false);
+      } else if (v.by_key) {
+        if (way == SP_UP) divide(w, v.khi + 1, v.khi0, v.above0, 0, want, false);
+        else divide(w, v.klo0, v.klo - 1, ab + in, 0, want, false);
+      } else {  // the bins just before, or just behind
+        need_bins();
+        const int b = way == SP_UP ? v.a - 1 : v.z + 1;
+        R.window_of(b, way == SP_UP ? 0 : b, way == SP_UP ? b : last, total, &v.a, &v.z);
+        set_bins(w);
+      }
       return 1;
     };
     int at;
@@ -1416,6 +1412,7 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
       many = p.n_above(SP_WINDOWS);
       left = p.above(SP_WINDOWS);
     }
+    win[SP_D].span.hi = min(win[SP_D].span.hi, many);
     double unused;
     if (cross(SP_D, (double)u * left, true, &at, &unused)) continue;
     found[SP_D] = true;

@@ -85,4 +85,36 @@ NVS_BOTH float sp_least_kept(float mx, float T, float min_p, double inv_t, C cou
          }));
 }
 
+// A crossing of a mass is looked for in windows, runs of values in the order. The mass
+// above a window and that of the values in it are sums of their own, added up in
+// another order than its neighbour's: where the crossing is an edge between two windows
+// up to rounding, the upper one may say that it is below and the lower one that it is
+// above. So what a window has said stays: the crossing is one of the values lo .. hi - 1
+// of the order, which only become fewer.
+struct SpSpan {
+  int lo, hi;
+};
+enum { SP_HERE, SP_UP, SP_DOWN };
+// Which way from a window of `in` values behind `above` others: past_above, past_through:
+// whether the mass above it, and with it, is past what is wanted. SP_HERE: the crossing
+// is one of the window's values (at least one of which is in the span then). SP_UP and
+// SP_DOWN exclude the window, and there are values on that side.
+NVS_BOTH int sp_turn(SpSpan& s, int above, int in, bool past_above, bool past_through) {
+  const int end = above + in;
+  if (in == 0) past_through = past_above;  // an empty window is never the place
+  if (past_above && above > s.lo) {
+    if (above < s.hi) s.hi = above;
+    return SP_UP;
+  }
+  if (!past_through && end < s.hi) {
+    if (end > s.lo) s.lo = end;
+    return SP_DOWN;
+  }
+  if (end <= s.lo) return SP_DOWN;
+  if (above >= s.hi) return SP_UP;
+  if (above > s.lo) s.lo = above;
+  if (end < s.hi) s.hi = end;
+  return SP_HERE;
+}
+
 }  // namespace nvs

@@ -1,8 +1,10 @@
 // The searches of csrc/sample_search.cuh on the host: what they find, and in how many steps.
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <random>
 #include <string>
+#include <vector>
 
 #include "sample_search.cuh"
 
@@ -62,8 +64,65 @@ static void least_kept_tests() {
   EXPECT(usual <= 3 * 100000, "an ordinary row takes two or three comparisons");
 }
 
+// A search over bins of values as the kernel does it: from a window of bins to its
+// neighbour on the side that sp_turn says. `past(n)`: whether the first n values' mass is
+// past what is wanted, as one pass has it; it may say something else in the next one.
+template <typename F>
+static int turns_of(const std::vector<int>& bins, int start, std::mt19937_64& g, F past, nvs::SpSpan* span, int* above,
+                    int* in) {
+  std::vector<int> before(1, 0);
+  for (int n : bins) before.push_back(before.back() + n);
+  int a = start, z = start;
+  *span = {0, before.back()};
+  for (int turn = 1;; ++turn) {
+    *above = before[a];
+    *in = before[z + 1] - before[a];
+    const bool past_above = past(*above), past_through = past(*above + *in);
+    const int way = nvs::sp_turn(*span, *above, *in, past_above, past_through);
+    if (way == nvs::SP_HERE || turn > 10000) return turn;
+    const int wide = (int)(g() % 3);
+    if (way == nvs::SP_UP) {
+      if (a == 0) return 20000;  // there is nothing
+      z = a - 1;
+      a = std::max(0, z - wide);
+    } else {
+      if (z + 1 == (int)bins.size()) return 20000;
+      a = z + 1;
+      z = std::min((int)bins.size() - 1, a + wide);
+    }
+  }
+}
+
+static void turn_tests() {
+  std::mt19937_64 g(9);
+  nvs::SpSpan span;
+  int above, in;
+  // two neighbours that disagree about the edge between them: the lower one decides
+  EXPECT(turns_of({5, 7, 6, 4}, 1, g, [&](int n) { return n >= 18 || (n == 12 && above == 12); }, &span, &above, &in) <= 3 &&
+             above == 12 && span.lo == 12, "an edge up to rounding");
+  for (int i = 0; i < 20000; ++i) {
+    std::vector<int> bins(1 + g() % 40);
+    int total = 0;
+    for (int& n : bins) total += n = g() % 3 ? (int)(g() % 9) : 0;
+    if (!total) continue;
+    const int start = (int)(g() % bins.size()), wanted = (int)(g() % total);
+    // sums that agree: the window that holds the crossing is found
+    int turns = turns_of(bins, start, g, [&](int n) { return n > wanted; }, &span, &above, &in);
+    EXPECT(turns <= (int)bins.size() && above <= wanted && wanted < above + in && span.lo <= wanted && wanted < span.hi,
+           "the crossing's window");
+    // sums that agree but for the crossing's own edge, which changes its mind
+    turns = turns_of(bins, start, g, [&](int n) { return n == wanted ? g() % 2 == 0 : n > wanted; }, &span, &above, &in);
+    EXPECT(turns <= (int)bins.size() + 2 && span.lo <= wanted && wanted <= span.hi, "an edge that changes its mind");
+    // whatever the sums say, it ends, in a window with a value that may be it
+    turns = turns_of(bins, start, g, [&](int) { return g() % 2 == 0; }, &span, &above, &in);
+    EXPECT(turns <= 2 * (int)bins.size() && above <= span.lo && span.lo < span.hi && span.hi <= above + in,
+           "any sums");
+  }
+}
+
 int main() {
   least_kept_tests();
+  turn_tests();
   std::printf("%d checks, %d failed\n", g_run, g_fail);
   return g_fail == 0 ? 0 : 1;
 }

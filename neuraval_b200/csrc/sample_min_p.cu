@@ -114,7 +114,7 @@ struct SpPart {
 
 struct SpShared {
   uint4 hist4[SP_BINS / 4];  // counts; in CTA 0, once merged, the counts before each bin
-  uint4 some4[SP_SOME / 4];  // the greatest key of each filled bin, of the first bins
+  uint4 some4[SP_SOME / 4];  // a value of each filled bin, of the first bins (sp_ticket)
   alignas(16) float mass[SP_BINS + 4];  // CTA 0, once merged: about the mass before each bin
   unsigned long long list[SP_WINDOWS * SP_CAP];
   SpCmd cmd;
@@ -141,6 +141,11 @@ struct SpShared {
 extern __shared__ uint4 sp_raw[];
 __device__ __forceinline__ SpShared& sp_shared() { return *reinterpret_cast<SpShared*>(sp_raw); }
 
+// A bin's stand-in is the value with the greatest ticket: as good as any of them, but not
+// one that depends on timing, since the order of the sums follows from what is guessed by
+// it. (The greatest value itself made the guesses too high: 5 us of 1024x151936 flat.)
+__device__ __forceinline__ uint32_t sp_ticket(float v) { return __brev(__float_as_uint(v)); }
+__device__ __forceinline__ float sp_drawn(uint32_t ticket) { return __uint_as_float(__brev(ticket)); }
 // A window's greatest key as a value. (No value has the key of -0; as a float it would
 // take +0 with it.)
 __device__ __forceinline__ float sp_edge(uint32_t k) {
@@ -537,8 +542,7 @@ struct SpRow {
         if (v[e] > -INFINITY) {
           const int b = k.bin(v[e]);
           atomicAdd(reinterpret_cast<int*>(s.hist4) + b, 1);
-          // (of some value: the windows that are guessed from it must not depend on timing)
-          if (b < SP_SOME) atomicMax(reinterpret_cast<uint32_t*>(s.some4) + b, sp_key(v[e]));
+          if (b < SP_SOME) atomicMax(reinterpret_cast<uint32_t*>(s.some4) + b, sp_ticket(v[e]));
         }
     });
   }
@@ -869,7 +873,7 @@ struct SpRow {
         const uint32_t fi[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (ci[j]) x[j] = sp_value(fi[j]);
+          if (ci[j]) x[j] = sp_drawn(fi[j]);
           n[j] += (int)ci[j];
         }
       }
@@ -1383,17 +1387,16 @@ __global__ void __launch_bounds__(SP_NT, 2) sample_min_p_kernel(const SpArgs a) 
         *mass = ab + (*at + 1.0) * wt;
         return 0;
       }
-      if (way == SP_HERE) {
-        divide(w, v.klo, v.khi, ab, above, want, false);
-      } else if (v.by_key) {
-        if (way == SP_UP) divide(w, v.khi + 1, v.khi0, v.above0, 0, want, false);
-        else divide(w, v.klo0, v.klo - 1, ab + in, 0, want, false);
-      } else {  // the bins just before, or just behind
+      if (way != SP_HERE && !v.by_key) {  // the bins just before, or just behind
         need_bins();
         const int b = way == SP_UP ? v.a - 1 : v.z + 1;
         R.window_of(b, way == SP_UP ? 0 : b, way == SP_UP ? b : last, total, &v.a, &v.z);
         set_bins(w);
+        return 1;
       }
+      const uint32_t lo = way == SP_UP ? v.khi + 1 : way == SP_DOWN ? v.klo0 : v.klo,
+                     hi = way == SP_UP ? v.khi0 : way == SP_DOWN ? v.klo - 1 : v.khi;
+      divide(w, lo, hi, way == SP_UP ? v.above0 : way == SP_DOWN ? ab + in : ab, 0, want, false);
       return 1;
     };
     int at;

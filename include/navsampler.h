@@ -392,10 +392,15 @@ typedef struct NcbAdapterHead NcbAdapterHead;
 NCB_API int ncb_adapter_head_create(int device, int dtype, int in_features, int out_features,
                                     int max_rows, int max_adapters, int max_rank,
                                     NcbAdapterHead** out);
-/* Waits for the device before it frees. Returns NCB_ERROR_LAUNCH_FAILED (and frees)
- * if a wait inside one of the handle's kernels ever gave up after its 2 s, which
- * leaves that call's output undefined. */
+/* Waits for the device before it frees. Returns what ncb_adapter_head_status would
+ * (and frees in any case). */
 NCB_API int ncb_adapter_head_destroy(NcbAdapterHead* head);
+/* NCB_ERROR_LAUNCH_FAILED if a wait inside one of the handle's kernels ever gave up
+ * after its 2 s, which leaves that call's output undefined; NCB_OK otherwise. A look
+ * at a word in host memory: it waits for nothing, so ask after the work of the calls in
+ * question has ended (the stream synchronised, say). From then on the handle projects
+ * no more: ncb_adapter_head_project_device returns the same error. */
+NCB_API int ncb_adapter_head_status(NcbAdapterHead* head);
 /* The shared weight, rows `ld` elements apart. It is read in place by later
  * calls and has to stay allocated, except where its base or row stride is not a
  * multiple of 16 bytes: then this call copies it (and allocates the copy, so

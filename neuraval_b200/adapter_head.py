@@ -112,5 +112,10 @@ class CudaAdapterHead:
             self._h, x.data_ptr(), ldx, rows, ids, out.data_ptr(), dtype_code(out.dtype), ldo,
             _stream_ptr(stream)), "ncb_adapter_head_project_device")
 
+    def check(self) -> None:
+        """NcbError if a wait inside one of the head's kernels gave up, which leaves that call's
+        output undefined. It waits for nothing: call it once the stream has been synchronised."""
+        check(self._lib.ncb_adapter_head_status(self._h), "ncb_adapter_head_status")
+
 
 __all__ = ["CudaAdapterHead"]

@@ -40,6 +40,7 @@
 #include <new>
 #include <type_traits>
 
+#include "bounded_wait.cuh"
 #include "navsampler.h"
 
 int ncb_record_status(int st);
@@ -96,7 +97,7 @@ struct AhArgs {
   int groups;  // tiles of rows worked on at the same time, by neighbouring CTAs
   uint32_t idesc, idesc_u;
   int stages;
-  uint32_t* error_word;
+  uint32_t* error_word;  // in host memory
 };
 
 // ---- loading a slot ---------------------------------------------------------------
@@ -403,27 +404,14 @@ __global__ void __launch_bounds__(AU_THREADS, 4) adapter_shrink_kernel(const AhA
 __device__ __forceinline__ uint32_t ah_smem(const void* p) {
   return (uint32_t)__cvta_generic_to_shared(p);
 }
-__device__ __forceinline__ bool ah_try(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok;
-}
-// Every wait ends: after about 2 s it gives up.
-__device__ __noinline__ bool ah_wait_long(uint32_t bar, uint32_t parity) {
-  uint64_t t0, t;
-  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
-  do {
-    if (ah_try(bar, parity)) return true;
-    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-  } while (t - t0 < 2000000000ull);
-  return false;
-}
+// Every wait ends: after 2 s it gives up.
 __device__ __forceinline__ bool ah_wait(uint32_t bar, uint32_t parity) {
-  return ah_try(bar, parity) || ah_try(bar, parity) || ah_wait_long(bar, parity);
+  return wait_for(bar, parity, 1000000000u);
+}
+// A wait gave up: a word in host memory, which the handle's calls look at.
+__device__ __forceinline__ void ah_failed(uint32_t* word, uint32_t where) {
+  *(volatile uint32_t*)word = where;
+  __threadfence_system();
 }
 __device__ __forceinline__ void ah_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
@@ -650,7 +638,7 @@ __global__ void __launch_bounds__(AH_THREADS, 1)
       }
     }
     if (!ok) {  // gave up: no copy may be in flight when the CTA ends
-      if (lane == 0) atomicOr(g.error_word, 1u);
+      if (lane == 0) ah_failed(g.error_word, 1u);
       for (int i = 0; rank == 0 && i < g.stages && i < issued; ++i) {
         if (s-- == 0) s = g.stages - 1, phase ^= 1;
         ah_wait(full + 8 * s, phase);
@@ -728,7 +716,7 @@ __global__ void __launch_bounds__(AH_THREADS, 1)
       if (!ok) {
         // products in flight end before TMEM is given back
         if (lane == 0) {
-          atomicOr(g.error_word, 2u);
+          ah_failed(g.error_word, 2u);
           ah_commit<CG>(done + 8 * (turn & 1));
         }
         ah_wait(done + 8 * (turn & 1), (turn >> 1) & 1);
@@ -793,7 +781,7 @@ __global__ void __launch_bounds__(AH_THREADS, 1)
         ++turn;
       }
     }
-    if (!ok && t == 0) atomicOr(g.error_word, 4u);
+    if (!ok && t == 0) ah_failed(g.error_word, 4u);
   }
   __syncwarp();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -816,13 +804,13 @@ struct NcbAdapterHead {
   int opad = 0;   // outputs, a multiple of 16
   int share = 0;  // outputs of a CTA: the same number for each, a multiple of 16
   std::mutex mu;
-  void* mem = nullptr;  // everything below but w and w_own
+  void* mem = nullptr;  // everything below but the error word, w and w_own
   void *a = nullptr, *b = nullptr, *u = nullptr, *x_own = nullptr;
   int32_t *ranks = nullptr, *counts = nullptr, *order = nullptr;
   int2* entries = nullptr;
   int4* info = nullptr;
   float* scales = nullptr;
-  uint32_t* error_word = nullptr;
+  uint32_t* error_word = nullptr;  // pinned: not 0 once a wait in a kernel has given up
   void* w_own = nullptr;  // the weight's copy, where it cannot be read in place
   bool has_w = false;
   const void* w = nullptr;  // what is read: the caller's weight or the copy
@@ -847,6 +835,9 @@ struct AhDevice {  // the handle's device for the duration of a call
 
 bool ah_aligned(const void* p, uintptr_t bytes) {
   return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
+}
+bool ah_gave_up(const NcbAdapterHead* h) {
+  return *static_cast<const volatile uint32_t*>(h->error_word) != 0;
 }
 int ah_launched() { return cudaGetLastError() == cudaSuccess ? NCB_OK : NCB_ERROR_LAUNCH_FAILED; }
 
@@ -1028,12 +1019,14 @@ NCB_API int ncb_adapter_head_create(int device, int dtype, int in_features, int 
   const size_t o_e = carve(tiles * most * sizeof(int2)), o_c = carve(tiles * 4);
   const size_t o_i = carve(tiles * nvs::AH_NT * sizeof(int4)), o_o = carve(tiles * nvs::AH_NT * 4);
   const size_t o_s = carve((size_t)h->slots * 4), o_r = carve((size_t)h->slots * 4);
-  const size_t o_w = carve(4);
-  if (cudaMalloc(&h->mem, off) != cudaSuccess) {
+  if (cudaMalloc(&h->mem, off) != cudaSuccess ||
+      cudaHostAlloc(&h->error_word, sizeof(uint32_t), cudaHostAllocMapped) != cudaSuccess) {
     cudaGetLastError();
+    cudaFree(h->mem);
     delete h;
     return ncb_record_status(NCB_ERROR_ALLOC_FAILED);
   }
+  *h->error_word = 0;
   char* m = static_cast<char*>(h->mem);
   h->a = m + o_a;
   h->b = m + o_b;
@@ -1045,8 +1038,8 @@ NCB_API int ncb_adapter_head_create(int device, int dtype, int in_features, int 
   h->counts = reinterpret_cast<int32_t*>(m + o_c);
   h->scales = reinterpret_cast<float*>(m + o_s);
   h->ranks = reinterpret_cast<int32_t*>(m + o_r);
-  h->error_word = reinterpret_cast<uint32_t*>(m + o_w);
-  bool ok = ah_share() && ah_raise() && cudaMemset(h->ranks, 0, off - o_r) == cudaSuccess &&
+  bool ok = ah_share() && ah_raise() &&
+            (!h->slots || cudaMemset(h->ranks, 0, (size_t)h->slots * 4) == cudaSuccess) &&
             cudaDeviceSynchronize() == cudaSuccess;
   if (ok && h->slots)  // 16 rows of 16 values are a row of the map
     ok = ah_map(&h->map_b, dtype, h->b, 256, (int64_t)per * h->opad / 256, 256, 256,
@@ -1054,6 +1047,7 @@ NCB_API int ncb_adapter_head_create(int device, int dtype, int in_features, int 
   if (!ok) {
     cudaGetLastError();
     cudaFree(h->mem);
+    cudaFreeHost(h->error_word);
     delete h;
     return ncb_record_status(NCB_ERROR_INIT_FAILED);
   }
@@ -1063,16 +1057,21 @@ NCB_API int ncb_adapter_head_create(int device, int dtype, int in_features, int 
 
 NCB_API int ncb_adapter_head_destroy(NcbAdapterHead* h) {
   if (!h) return ncb_record_status(NCB_ERROR_INVALID_ARGUMENT);
-  uint32_t error = 0;
+  bool error = false;
   {
     AhDevice guard(h->device);
-    cudaDeviceSynchronize();
-    if (cudaMemcpy(&error, h->error_word, sizeof(error), cudaMemcpyDeviceToHost) != cudaSuccess) error = 1;
+    error = cudaDeviceSynchronize() != cudaSuccess || ah_gave_up(h);
     cudaFree(h->mem);
     cudaFree(h->w_own);
+    cudaFreeHost(h->error_word);
   }
   delete h;
   return ncb_record_status(error ? NCB_ERROR_LAUNCH_FAILED : NCB_OK);
+}
+
+NCB_API int ncb_adapter_head_status(NcbAdapterHead* h) {
+  if (!h) return ncb_record_status(NCB_ERROR_NOT_INITIALIZED);
+  return ncb_record_status(ah_gave_up(h) ? NCB_ERROR_LAUNCH_FAILED : NCB_OK);
 }
 
 NCB_API int ncb_adapter_head_set_weight_device(NcbAdapterHead* h, const void* d_weight, int64_t ld,
@@ -1145,6 +1144,7 @@ NCB_API int ncb_adapter_head_project_device(NcbAdapterHead* h, const void* d_x, 
       !ah_aligned(d_out, out_dtype == NCB_DTYPE_F32 ? 4 : 2) || !ah_aligned(d_adapter_ids, 4))
     return ncb_record_status(NCB_ERROR_INVALID_ARGUMENT);
   if (rows > h->max_rows) return ncb_record_status(NCB_ERROR_CAPACITY);
+  if (ah_gave_up(h)) return ncb_record_status(NCB_ERROR_LAUNCH_FAILED);
   std::lock_guard<std::mutex> lk(h->mu);
   AhDevice guard(h->device);
   if (!guard.ok) return ncb_record_status(NCB_ERROR_INIT_FAILED);

@@ -321,6 +321,9 @@ class AdapterHead {
     check(ncb_adapter_head_clear_adapter_device(h_, slot, stream),
           "ncb_adapter_head_clear_adapter_device");
   }
+  // CudaException if a wait inside one of the head's kernels gave up; to be called once
+  // the stream has been synchronised.
+  void Check() const { check(ncb_adapter_head_status(h_), "ncb_adapter_head_status"); }
   // out [rows, outFeatures] of outDtype from x [rows, inFeatures]; adapterIds: a slot
   // per row (-1: none), or nullptr.
   void Project(const void* x, int64_t ldx, int rows, const int32_t* adapterIds, void* out,
@@ -546,6 +549,7 @@ class TextGenerator {
       cuda(cudaMemcpyAsync(h + 6 * rows, d + 6 * rows, 4 * rows, cudaMemcpyDeviceToHost, stream),
            "cudaMemcpyAsync");
       cuda(cudaStreamSynchronize(stream), "cudaStreamSynchronize");
+      head.Check();
       std::vector<size_t> still;
       for (size_t j = 0; j < rows; ++j) {
         const size_t i = running[j];

@@ -94,6 +94,7 @@ SIGNATURES = {
                                           _P]),
     "ncb_adapter_head_create": (_I, [_I, _I, _I, _I, _I, _I, _I, ctypes.POINTER(_P)]),
     "ncb_adapter_head_destroy": (_I, [_P]),
+    "ncb_adapter_head_status": (_I, [_P]),
     "ncb_adapter_head_set_weight_device": (_I, [_P, _P, _L, _P]),
     "ncb_adapter_head_set_adapter_device": (_I, [_P, _I, _P, _L, _P, _L, _I, _F, _P]),
     "ncb_adapter_head_clear_adapter_device": (_I, [_P, _I, _P]),

@@ -151,6 +151,10 @@ class DefaultRandom final : public Random {
   std::mt19937_64 gen_;
 };
 
+// A draw as ncb_sample_rows_min_p_device takes it, in [0, 1): doubles from 1 - 2^-25 on
+// would round to 1.
+inline float UniformBelowOne(double u) { return std::min(static_cast<float>(u), 1.0f - 0x1p-24f); }
+
 // One GPU's sampler handle (ncb_sampler_create): scratch for up to maxRows rows
 // of up to maxVocab columns and maxHistory generated ids per row.
 class Device {
@@ -529,7 +533,7 @@ class TextGenerator {
         const BatchRequest& r = requests[running[j]];
         const bool greedy = r.Options.Greedy();
         const float T = greedy ? 0.0f : r.Options.Temperature(), top_p = r.Options.TopP(),
-                    u = greedy ? 0.0f : static_cast<float>(random[running[j]]->NextDouble());
+                    u = greedy ? 0.0f : UniformBelowOne(random[running[j]]->NextDouble());
         h[j] = r.Adapter;
         std::memcpy(h + rows + j, &T, 4);
         h[2 * rows + j] = r.Options.TopK();

@@ -1,0 +1,124 @@
+// TextGenerator::GenerateBatch where something goes wrong for one request, or for all: the
+// largest draws, rows without a token, a head whose kernel gave up. `--no-gpu` runs what
+// needs no GPU.
+#include <cmath>
+#include <cstdio>
+#include <cstring>
+#include <string>
+#include <vector>
+
+#include <cuda_fp16.h>
+
+#include "neuraval_generation.hpp"
+
+using namespace neuraval;
+
+static int g_fail = 0, g_run = 0;
+#define EXPECT(cond, what)                                                     \
+  do {                                                                         \
+    ++g_run;                                                                   \
+    if (!(cond)) {                                                             \
+      ++g_fail;                                                                \
+      std::fprintf(stderr, "FAIL %s: %s\n", std::string(what).c_str(), #cond); \
+    }                                                                          \
+  } while (0)
+
+// Stands in for the library's: what the head's kernels are said to have come to.
+static int g_status = NCB_OK;
+extern "C" int ncb_adapter_head_status(NcbAdapterHead*) { return g_status; }
+
+struct Fixed final : Random {
+  double u;
+  explicit Fixed(double v) : u(v) {}
+  double NextDouble() override { return u; }
+};
+
+static void draw_tests() {
+  EXPECT(UniformBelowOne(0.0) == 0.0f && UniformBelowOne(0.3) == 0.3f, "ordinary draws as they are");
+  for (double u : {1.0 - 0x1p-24, 1.0 - 0x1p-25, 1.0 - 0x1p-26, 1.0 - 0x1p-53})
+    EXPECT(UniformBelowOne(u) == 1.0f - 0x1p-24f, "the largest draws stay below 1");
+}
+
+constexpr int IN = 32, V = 300, ROWS = 8;
+static int small(uint64_t z) {
+  z = z * 0x9E3779B97F4A7C15ull + 0x1234567ull;
+  z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+  return static_cast<int>((z ^ (z >> 27)) % 5) - 2;
+}
+struct Buffer {
+  void* p = nullptr;
+  explicit Buffer(size_t bytes) {
+    if (cudaMalloc(&p, bytes) != cudaSuccess) throw CudaException(NCB_ERROR_ALLOC_FAILED, "cudaMalloc");
+  }
+  ~Buffer() { cudaFree(p); }
+  void fill(const std::vector<__half>& h) { cudaMemcpy(p, h.data(), h.size() * 2, cudaMemcpyHostToDevice); }
+};
+
+// A head with sound adapters in slot 0 and one with a NaN in slot 1, and a toy model whose
+// hidden state is NaN for contexts that begin with `poisoned` and have `from` tokens or more.
+struct Bench {
+  cudaStream_t st = nullptr;
+  Device dev{0, 1, V, 16};
+  AdapterHead head{0, NCB_DTYPE_F16, IN, V, ROWS, 2, 4};
+  Buffer w{2 * V * IN}, a{2 * 4 * IN}, b{2 * V * 4}, x{2 * ROWS * IN};
+  TextGenerator gen{dev, 64};
+  int poisoned = -1;
+  size_t from = 0;
+  Bench() {
+    cudaStreamCreate(&st);
+    std::vector<__half> h;
+    for (int i = 0; i < V * IN; ++i) h.push_back(__float2half(small(i) / 8.0f));
+    w.fill(h);
+    head.SetWeight(w.p, IN, st);
+    for (int slot = 0; slot < 2; ++slot) {
+      h.clear();
+      for (int i = 0; i < 4 * IN; ++i) h.push_back(__float2half(small(7000 + i) / 8.0f));
+      a.fill(h);
+      h.clear();
+      for (int i = 0; i < V * 4; ++i) h.push_back(__float2half(small(9000 + i) / 8.0f));
+      if (slot == 1) h[77] = __float2half(NAN);
+      b.fill(h);
+      head.SetAdapter(slot, a.p, IN, b.p, 4, 4, 0.5f, st);
+      cudaStreamSynchronize(st);
+    }
+  }
+  ~Bench() { cudaStreamDestroy(st); }
+  std::vector<GenerationResult> run(const std::vector<BatchRequest>& rq, const std::vector<Random*>& randoms = {}) {
+    return gen.GenerateBatch(
+        [this](const std::vector<std::vector<int>>& contexts, cudaStream_t stream) {
+          std::vector<__half> rows;
+          for (const auto& c : contexts) {
+            uint64_t z = 0;
+            for (int t : c) z = z * 31 + t + 1;
+            const bool bad = c[0] == poisoned && c.size() >= from;
+            for (int i = 0; i < IN; ++i) rows.push_back(__float2half(bad ? NAN : static_cast<float>(small(z + i))));
+          }
+          cudaMemcpyAsync(x.p, rows.data(), rows.size() * 2, cudaMemcpyHostToDevice, stream);
+          cudaStreamSynchronize(stream);
+          return static_cast<const void*>(x.p);
+        },
+        head, rq, st, randoms);
+  }
+};
+
+static const std::vector<int> none;
+static GenerationOptions sampled(int seed, float T = 0.9f) {
+  return GenerationOptions::Create(false, T, 0.95f, 40, 1.0f, 12, none, seed);
+}
+
+static void largest_draw(Bench& t) {
+  Fixed top(1.0 - 0x1p-26), low(0.25);
+  const auto r = t.run({{{3, 1}, sampled(1), 0.0f, 0}, {{4}, sampled(2), 0.0f, -1}}, {&top, &low});
+  EXPECT(r[0].GeneratedTokenIds.size() == 12 && r[1].GeneratedTokenIds.size() == 12, "a draw next to 1 gives a token");
+  for (int token : r[0].GeneratedTokenIds) EXPECT(token >= 0 && token < V, "a token of the vocabulary");
+}
+
+int main(int argc, char** argv) {
+  draw_tests();
+  if (argc < 2 || std::strcmp(argv[1], "--no-gpu") != 0) {
+    Bench t;
+    largest_draw(t);
+  }
+  std::printf("%d checks, %d failed\n", g_run, g_fail);
+  return g_fail == 0 ? 0 : 1;
+}

@@ -351,11 +351,14 @@ struct BatchRequest {
 };
 
 // GenerationFinishReason (GenerationFinishReason.cs) and GenerationResult
-// (GenerationResult.cs:7-27).
-enum class GenerationFinishReason { MaxNewTokens, StopToken };
+// (GenerationResult.cs:7-27). Failed and Flags are GenerateBatch's, for a request that
+// ended without a token to go on with: NCB_FLAG_NONFINITE or NCB_FLAG_BAD_OPTIONS. The
+// tokens before that are there.
+enum class GenerationFinishReason { MaxNewTokens, StopToken, Failed };
 struct GenerationResult {
   std::vector<int> GeneratedTokenIds;
   GenerationFinishReason FinishReason = GenerationFinishReason::MaxNewTokens;
+  uint32_t Flags = 0;
 };
 
 // TextGenerator.Generate (TextGenerator.cs:19-51): the decode loop around
@@ -472,11 +475,13 @@ class TextGenerator {
   // Generate for many requests in step, each with options, random source and
   // adapter of its own: per step the model's hidden states of the requests still
   // running, the head's projection with their adapters and one sampling call with
-  // their options; 24 bytes per request go to the device and 4 come back.
+  // their options; 24 bytes per request go to the device and 8 come back.
   // `randoms`: a source per request, or empty (each request then seeds its own).
-  // A request's tokens do not depend on the others'. Repetition, frequency and
-  // presence penalties are one value per call in the library, so a request that
-  // sets one is refused.
+  // A request's tokens do not depend on the others': one whose logits are not finite
+  // (its hidden state, its adapter, a product past fp16's range) or whose options the
+  // sampling call does not take ends as Failed, alone. ncb_sample_rows_min_p_device
+  // knows no history of tokens, so a request that sets a repetition, frequency or
+  // presence penalty (GenerationOptions::Default does) is refused; Generate takes it.
   std::vector<GenerationResult> GenerateBatch(const HiddenModel& model, const AdapterHead& head,
                                               const std::vector<BatchRequest>& requests,
                                               cudaStream_t stream,
@@ -500,15 +505,15 @@ class TextGenerator {
     std::unique_ptr<void, decltype(restore)> device(this_address(), restore);
     auto dev_free = [](void* p) { cudaFree(p); };
     auto host_free = [](void* p) { cudaFreeHost(p); };
-    // per request: adapter, T, top_k, top_p, min_p, u; then the token
+    // per request: adapter, T, top_k, top_p, min_p, u; then the token and its flags
     void* p = nullptr;
-    cuda(cudaMalloc(&p, 7 * 4 * n), "cudaMalloc");
+    cuda(cudaMalloc(&p, 8 * 4 * n), "cudaMalloc");
     std::unique_ptr<void, decltype(dev_free)> dmem(p, dev_free);
     p = nullptr;
     cuda(cudaMalloc(&p, sizeof(float) * n * vocab), "cudaMalloc");
     std::unique_ptr<void, decltype(dev_free)> logits(p, dev_free);
     p = nullptr;
-    cuda(cudaMallocHost(&p, 7 * 4 * n), "cudaMallocHost");
+    cuda(cudaMallocHost(&p, 8 * 4 * n), "cudaMallocHost");
     std::unique_ptr<void, decltype(host_free)> hmem(p, host_free);
     int32_t* d = static_cast<int32_t*>(dmem.get());
     int32_t* h = static_cast<int32_t*>(hmem.get());
@@ -548,9 +553,10 @@ class TextGenerator {
       check(ncb_sample_rows_min_p_device(logits.get(), NCB_DTYPE_F32, static_cast<int>(rows),
                                          static_cast<int>(vocab), static_cast<int64_t>(vocab),
                                          f + 5 * rows, f + rows, d + 2 * rows, f + 3 * rows,
-                                         f + 4 * rows, d + 6 * rows, nullptr, nullptr, nullptr, stream),
+                                         f + 4 * rows, d + 6 * rows, nullptr, nullptr,
+                                         reinterpret_cast<uint32_t*>(d + 7 * rows), stream),
             "ncb_sample_rows_min_p_device");
-      cuda(cudaMemcpyAsync(h + 6 * rows, d + 6 * rows, 4 * rows, cudaMemcpyDeviceToHost, stream),
+      cuda(cudaMemcpyAsync(h + 6 * rows, d + 6 * rows, 2 * 4 * rows, cudaMemcpyDeviceToHost, stream),
            "cudaMemcpyAsync");
       cuda(cudaStreamSynchronize(stream), "cudaStreamSynchronize");
       head.Check();
@@ -558,7 +564,11 @@ class TextGenerator {
       for (size_t j = 0; j < rows; ++j) {
         const size_t i = running[j];
         const int next = h[6 * rows + j];
-        if (next < 0) throw CudaException(NCB_ERROR_INVALID_ARGUMENT, "GenerateBatch: row not sampled");
+        if (next < 0) {
+          results[i].FinishReason = GenerationFinishReason::Failed;
+          results[i].Flags = static_cast<uint32_t>(h[7 * rows + j]);
+          continue;
+        }
         results[i].GeneratedTokenIds.push_back(next);
         sequences[i].push_back(next);
         if (IsStop(requests[i].Options, next))

@@ -113,11 +113,54 @@ static void largest_draw(Bench& t) {
   for (int token : r[0].GeneratedTokenIds) EXPECT(token >= 0 && token < V, "a token of the vocabulary");
 }
 
+static bool same(const GenerationResult& a, const GenerationResult& b) {
+  return a.GeneratedTokenIds == b.GeneratedTokenIds && a.FinishReason == b.FinishReason && a.Flags == b.Flags;
+}
+
+static void one_of_many(Bench& t) {
+  const std::vector<BatchRequest> sound = {{{3, 1}, sampled(1), 0.0f, 0},
+                                           {{4}, GenerationOptions::CreateGreedy(9, none), 0.0f, -1},
+                                           {{5, 5}, sampled(3), 0.1f, 0}};
+  const auto want = t.run(sound);
+  for (const auto& r : want) EXPECT(r.FinishReason == GenerationFinishReason::MaxNewTokens && r.Flags == 0, "sound requests");
+  // an adapter with a NaN, a hidden state that becomes NaN, and options out of range, among them
+  t.poisoned = 250;
+  t.from = 4;
+  std::vector<BatchRequest> rq = {sound[0], {{8, 2}, sampled(4), 0.0f, 1}, sound[1], {{250}, sampled(5), 0.0f, 0}, sound[2],
+                                  {{6}, sampled(6, NAN), 0.0f, -1}, {{7}, GenerationOptions::CreateGreedy(3, none), 0.0f, 1}};
+  const auto r = t.run(rq);
+  EXPECT(same(r[0], want[0]) && same(r[2], want[1]) && same(r[4], want[2]), "the others' tokens are as without them");
+  for (size_t i : {size_t{1}, size_t{6}})
+    EXPECT(r[i].FinishReason == GenerationFinishReason::Failed && r[i].Flags == NCB_FLAG_NONFINITE &&
+               r[i].GeneratedTokenIds.empty(), "an adapter with a NaN fails its request");
+  EXPECT(r[3].FinishReason == GenerationFinishReason::Failed && r[3].Flags == NCB_FLAG_NONFINITE &&
+             r[3].GeneratedTokenIds.size() == 3, "a request that fails later keeps its tokens");
+  EXPECT(r[5].FinishReason == GenerationFinishReason::Failed && r[5].Flags == NCB_FLAG_BAD_OPTIONS, "options out of range");
+  t.poisoned = -1;
+  const auto alone = t.run({rq[1]});
+  EXPECT(alone.size() == 1 && alone[0].FinishReason == GenerationFinishReason::Failed, "the last request running fails");
+}
+
+static void a_kernel_gave_up(Bench& t) {
+  g_status = NCB_ERROR_LAUNCH_FAILED;
+  int status = NCB_OK;
+  try {
+    t.run({{{3, 1}, sampled(1), 0.0f, 0}});
+  } catch (const CudaException& e) {
+    status = e.status;
+  }
+  EXPECT(status == NCB_ERROR_LAUNCH_FAILED, "undefined logits are not sampled on");
+  g_status = NCB_OK;
+  EXPECT(t.run({{{3, 1}, sampled(1), 0.0f, 0}})[0].GeneratedTokenIds.size() == 12, "and as before without");
+}
+
 int main(int argc, char** argv) {
   draw_tests();
   if (argc < 2 || std::strcmp(argv[1], "--no-gpu") != 0) {
     Bench t;
     largest_draw(t);
+    one_of_many(t);
+    a_kernel_gave_up(t);
   }
   std::printf("%d checks, %d failed\n", g_run, g_fail);
   return g_fail == 0 ? 0 : 1;

@@ -515,6 +515,9 @@ class TextGenerator {
     p = nullptr;
     cuda(cudaMallocHost(&p, 8 * 4 * n), "cudaMallocHost");
     std::unique_ptr<void, decltype(host_free)> hmem(p, host_free);
+    // an exception may leave copies on the stream: they end before their buffers do
+    const auto wait = [stream](void*) { cudaStreamSynchronize(stream); };
+    std::unique_ptr<void, decltype(wait)> idle(this_address(), wait);
     int32_t* d = static_cast<int32_t*>(dmem.get());
     int32_t* h = static_cast<int32_t*>(hmem.get());
     std::vector<std::optional<DefaultRandom>> own(n);

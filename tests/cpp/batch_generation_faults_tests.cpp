@@ -1,10 +1,14 @@
 // TextGenerator::GenerateBatch where something goes wrong for one request, or for all: the
 // largest draws, rows without a token, a head whose kernel gave up. `--no-gpu` runs what
 // needs no GPU.
+#include <dlfcn.h>
+
+#include <chrono>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <string>
+#include <thread>
 #include <vector>
 
 #include <cuda_fp16.h>
@@ -26,6 +30,20 @@ static int g_fail = 0, g_run = 0;
 // Stands in for the library's: what the head's kernels are said to have come to.
 static int g_status = NCB_OK;
 extern "C" int ncb_adapter_head_status(NcbAdapterHead*) { return g_status; }
+
+// And this one refuses when it is told to, behind work that takes its time.
+static bool g_refuse = false, g_ended = false;
+extern "C" int ncb_sample_rows_min_p_device(const void* logits, int dtype, int rows, int vocab, int64_t ld, const float* u,
+                                            const float* T, const int32_t* k, const float* p, const float* m,
+                                            int32_t* tokens, float* lp, int32_t* kept, uint32_t* flags, void* stream) {
+  static const auto next = reinterpret_cast<decltype(&ncb_sample_rows_min_p_device)>(dlsym(RTLD_NEXT, "ncb_sample_rows_min_p_device"));
+  if (!g_refuse) return next(logits, dtype, rows, vocab, ld, u, T, k, p, m, tokens, lp, kept, flags, stream);
+  cudaLaunchHostFunc(static_cast<cudaStream_t>(stream), [](void*) {
+    std::this_thread::sleep_for(std::chrono::milliseconds(50));
+    g_ended = true;
+  }, nullptr);
+  return NCB_ERROR_CAPACITY;
+}
 
 struct Fixed final : Random {
   double u;
@@ -154,6 +172,18 @@ static void a_kernel_gave_up(Bench& t) {
   EXPECT(t.run({{{3, 1}, sampled(1), 0.0f, 0}})[0].GeneratedTokenIds.size() == 12, "and as before without");
 }
 
+static void a_refused_call(Bench& t) {
+  g_refuse = true;
+  int status = NCB_OK;
+  try {
+    t.run({{{3, 1}, sampled(1), 0.0f, 0}});
+  } catch (const CudaException& e) {
+    status = e.status;
+  }
+  g_refuse = false;
+  EXPECT(status == NCB_ERROR_CAPACITY && g_ended && cudaStreamQuery(t.st) == cudaSuccess, "nothing is left on the stream");
+}
+
 int main(int argc, char** argv) {
   draw_tests();
   if (argc < 2 || std::strcmp(argv[1], "--no-gpu") != 0) {
@@ -161,6 +191,7 @@ int main(int argc, char** argv) {
     largest_draw(t);
     one_of_many(t);
     a_kernel_gave_up(t);
+    a_refused_call(t);
   }
   std::printf("%d checks, %d failed\n", g_run, g_fail);
   return g_fail == 0 ? 0 : 1;

@@ -19,7 +19,7 @@ def _build(tmp_path):
                     "-I", os.path.join(CUDA, "include"),
                     os.path.join(ROOT, "tests", "cpp", "batch_generation_faults_tests.cpp"),
                     "-L", libdir, "-lnavsampler", f"-Wl,-rpath,{libdir}",
-                    "-L", os.path.join(CUDA, "lib64"), "-lcudart", f"-Wl,-rpath,{os.path.join(CUDA, 'lib64')}",
+                    "-L", os.path.join(CUDA, "lib64"), "-lcudart", "-ldl", f"-Wl,-rpath,{os.path.join(CUDA, 'lib64')}",
                     "-o", str(exe)], check=True)
     return exe
 

@@ -373,10 +373,13 @@ NCB_API int ncb_sample_rows_min_p_device(const void* d_logits, int dtype, int ro
  * W is [out_features, in_features], A_s [rank_s, in_features], B_s
  * [out_features, rank_s], x [rows, in_features], all of the handle's dtype
  * (NCB_DTYPE_F16 or NCB_DTYPE_BF16). Products are summed in fp32 and rounded
- * once, to the output's type; scale_s A_s x_n goes into the second product as the
- * sum of two values of the handle's type (2^-16 of it or less is lost), of three
- * where bf16 is projected to fp32 (2^-24). No sum's order depends on timing: the
- * same call gives the same bits. A row whose adapter holds a NaN or an infinity,
+ * once, to the output's type; u = scale_s A_s x_n goes into the second product as the
+ * sum of two values of the handle's type, of three where bf16 is projected to fp32.
+ * Lost of each value of u: bf16 2^-16 of it (2^-24 with three); fp16 2^-22 of it, but
+ * 2^-25 where it is below 2^-3, since the type has no smaller steps than 2^-24: more than
+ * 2^-16 of it below 2^-9, all of it below 2^-25. (Where u is that small and B is not, move a
+ * power of two from B to A, or keep the head in bf16.) No sum's order depends on timing:
+ * the same call gives the same bits. A row whose adapter holds a NaN or an infinity,
  * or whose scale_s A_s x_n is not finite in the handle's type (fp16: beyond
  * 65504), comes back as NaN; no other row of the call is touched by it.
  *

@@ -10,7 +10,9 @@
 // and zeros for the others, split into 16-bit values, each with its own product (one
 // would round u to 8 bits of bf16): two, u = hi + lo, 16 bits, where the output is
 // rounded to fewer anyway, and three for bf16 with an fp32 output (with two the
-// result was 1.2e-6 off, more than all of the sums).
+// result was 1.2e-6 off, more than all of the sums). fp16 has 22 bits in two, but none
+// below 2^-24, so what is lost of a small u is 2^-25 instead; a third value would not
+// change that, and B in a wider type would double its bytes and its products.
 //
 // Tiles of up to AH_SINGLE rows have one block, the tile. Larger tiles are sorted by
 // slot first (adapter_sort_kernel copies x in that order) and cut into blocks of 32

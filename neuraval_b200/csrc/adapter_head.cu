@@ -27,9 +27,10 @@
 // head waits for it only before the first entry (programmatic dependent launch).
 //
 // Up to about 256 rows the head is bound by the weight's bytes (32x4096x128256, 8
-// slots of 16 ranks: 176 us, 6.2 TB/s), beyond by the tensor cores and the power they
-// draw (512x4096x151936, 16 slots of 32 ranks: 582 us alone, 1.1 PFLOP/s, 700 us in
-// a long loop whose clock sinks to 1 GHz).
+// slots of 16 ranks, fp32 output: 183 us in a short loop, 191 in a long one, 5.8 TB/s;
+// without adapters 170), beyond by the tensor cores and the power they draw
+// (512x4096x151936, 16 slots of 32 ranks: 636 us alone, 1.0 PFLOP/s, 748 us in a long
+// loop whose clock sinks to 1 GHz; without adapters 474 and 576).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -33,9 +33,11 @@
 //
 // Keeping a cluster's slices of the row in shared memory, for one read in all, was
 // slower: it leaves two CTAs per SM in long chains of small steps, and more of them
-// per row to synchronise (1024x151936 with top-p alone: 2.3 ms, now 0.94, of which
+// per row to synchronise (1024x151936 with top-p alone: 2.3 ms, now 0.95, of which
 // the 64-bit weights of the exact pass are the largest part: it issues about 30
-// operations per value).
+// operations per value). A crossing in a bin of more than SP_CAP values takes up to seven
+// passes: one row in a hundred of 256x128256 with top-p alone, peaked at few values,
+// which then decide how long the call takes (1.4 ms).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -61,7 +63,10 @@ constexpr int SP_CAP = 512;      // and one window's part of the list
 constexpr int SP_WIDEN = 96;     // values up to which a guessed window takes in its neighbours
 constexpr int SP_RANKED = 256;   // lists up to this are sorted by ranks
 constexpr int SP_SOME = 512;     // bins of which a value is kept, for the guess
-constexpr int SP_BOUNDED = 256;  // largest top_k that the threads' maxima bound
+// Largest top_k that the threads' maxima bound: half of a CTA's threads (with hardly more
+// maxima than values wanted the bound is so low that the list overflows). 256x128256 fp32, all rows alike: top_k 50 55 us, 256 72; from
+// 257 on the histogram decides, 110 us, 121 for 1000.
+constexpr int SP_BOUNDED = 256;
 constexpr int SP_CLUSTER = 8;    // largest cluster
 constexpr int SP_TURNS = 4096;   // passes over a row at most
 constexpr int SP_MAX_VOCAB = 1 << 24;
@@ -1925,6 +1930,11 @@ int sp_launch(const nvs::SpArgs& a, int rows, int device, int num_sms, cudaStrea
     // as many CTAs to a row as its values need, then as fill the GPU, one per SM
     // (their counters take its shared memory). Each counts up to 65535 values: 128256
     // values need two, which 256 rows' 512 CTAs pay for with 3.5 waves.
+    // The options are on the device, so the choice is by size. Counting takes the same
+    // time whatever they are; the kernel of the lists, which longer rows take, is faster
+    // where few values are wanted and far slower where it has to guess (256x128256 bf16,
+    // counts and lists: top_k 50 106 and 49 us, 300 107 and 88, 1000 107 and 179, top_p
+    // alone 107 and 1435, greedy 91 and 71).
     const int values = granules * n;
     int ranks = values <= nvs::SQ_ALONE ? 1 : 2;
     while (ranks < nvs::SP_CLUSTER &&

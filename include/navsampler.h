@@ -407,7 +407,9 @@ NCB_API int ncb_adapter_head_status(NcbAdapterHead* head);
 /* The shared weight, rows `ld` elements apart. It is read in place by later
  * calls and has to stay allocated, except where its base or row stride is not a
  * multiple of 16 bytes: then this call copies it (and allocates the copy, so
- * not while a stream is captured). Call it again after changing the weight. */
+ * not while a stream is captured). Call it again after changing the weight. Captured
+ * calls keep reading the weight they were captured with (a copy, which is overwritten
+ * in place, or the caller's memory, which has to stay). */
 NCB_API int ncb_adapter_head_set_weight_device(NcbAdapterHead* head, const void* d_weight,
                                                int64_t ld, void* stream);
 /* Copies adapter `slot` in (1 <= rank <= max_rank, finite scale): d_a

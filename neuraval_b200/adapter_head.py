@@ -64,7 +64,8 @@ class CudaAdapterHead:
             pass
 
     def set_weight(self, weight, stream=None) -> None:
-        """The shared weight, same shape, type and device as the one the head was made with."""
+        """The shared weight, same shape, type and device as the one the head was made with. The
+        head holds on to this tensor only: graphs captured with an earlier one still read that."""
         if weight.shape[0] != self.out_features:
             raise ValueError(f"weight must have {self.out_features} rows")
         ld = _rows_of(weight, "weight", self.in_features, self.dtype, self.device)
